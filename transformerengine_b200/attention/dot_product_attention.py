@@ -41,8 +41,13 @@ class DotProductAttention(torch.nn.Module):
                  cp_global_ranks: Optional[List[int]] = None, cp_stream=None, cp_comm_type: str = "p2p",
                  softmax_scale: Optional[float] = None, softmax_type: str = "vanilla",
                  return_max_logit: bool = False, bottom_right_diagonal: Optional[bool] = None,
-                 name: Optional[str] = None) -> None:
+                 name: Optional[str] = None, sink_tokens: int = 0) -> None:
+        """``sink_tokens``: first tokens of every sequence that stay visible left of the sliding window (streaming
+        attention).  It has no effect without a window; ``softmax_type="learnable"`` is another kind of sink."""
         super().__init__()
+        if sink_tokens < 0:
+            raise ValueError("sink_tokens must not be negative")
+        self.sink_tokens = sink_tokens
         self.bottom_right_diagonal, self.name = bottom_right_diagonal, name
         # return_max_logit: forward returns (output, per-head maximum of the masked scaled scores); the maximum
         # comes from a pass of its own over Q K^T (the attention kernels do not export it)
@@ -247,6 +252,7 @@ class DotProductAttention(torch.nn.Module):
                 ("score_mod", score[0] is not None),
                 ("bottom-right causal alignment with sq != sk", causal and bottom_right and sq != sk),
                 ("return_max_logit", self.return_max_logit),
+                ("sink_tokens", self.sink_tokens > 0 and windowed),
             ) if on]
             if unsupported:
                 raise NotImplementedError("context parallelism does not support: " + "; ".join(unsupported))
@@ -261,13 +267,14 @@ class DotProductAttention(torch.nn.Module):
                     raise NotImplementedError("return_max_logit with score_mod")
                 from ..ops.attention import max_attention_logit
                 self._max_logit = max_attention_logit(qb, kb, scale=self.softmax_scale, causal=causal, window=window,
-                                                      attn_mask=mask, bias=the_bias,
+                                                      attn_mask=mask, bias=the_bias, sink_tokens=self.sink_tokens,
                                                       bottom_right=bottom_right or sq == sk)
             with ctx:
                 o = ops.attention(qb, kb, vb, scale=self.softmax_scale, causal=causal, window=window, attn_mask=mask,
                                   bias=the_bias, dropout_p=dropout, softmax_type=self.softmax_type,
                                   sink=self.softmax_offset, bottom_right=bottom_right or sq == sk,
-                                  out_format=fmt, score_mod=score[0], score_mod_tensors=score[1])
+                                  out_format=fmt, score_mod=score[0], score_mod_tensors=score[1],
+                                  sink_tokens=self.sink_tokens)
         if fmt == "sbhd":
             return o.permute(2, 0, 1, 3).reshape(sq, b, hq * o.shape[-1])
         return o.permute(0, 2, 1, 3).reshape(b, sq, hq * o.shape[-1])
@@ -304,7 +311,8 @@ class DotProductAttention(torch.nn.Module):
             o = flash.flash_attention_varlen(q, k, v, cu_q, cu_kv, scale=self.softmax_scale, causal=causal,
                                              bottom_right="bottom_right" in mask_type, max_seqlen_q=max_sq,
                                              max_seqlen_kv=max_skv, cu_seqlens_q_padded=cu_q_padded,
-                                             cu_seqlens_kv_padded=cu_kv_padded, window=window)
+                                             cu_seqlens_kv_padded=cu_kv_padded, window=window,
+                                             sink_tokens=self.sink_tokens)
             return o.reshape(o.shape[0], -1)
         cq, ck = cu_q.tolist(), cu_kv.tolist()
         oq = cq if cu_q_padded is None else cu_q_padded.tolist()
@@ -318,7 +326,7 @@ class DotProductAttention(torch.nn.Module):
             ki = k[ok_[i]:ok_[i] + lk].permute(1, 0, 2).unsqueeze(0)
             vi = v[ok_[i]:ok_[i] + lk].permute(1, 0, 2).unsqueeze(0)
             o = ops.attention(qi, ki, vi, scale=self.softmax_scale, causal=causal, window=window,
-                              softmax_type=self.softmax_type, sink=self.softmax_offset,
+                              softmax_type=self.softmax_type, sink=self.softmax_offset, sink_tokens=self.sink_tokens,
                               bottom_right="bottom_right" in mask_type or lq == lk)
             o = o.squeeze(0).permute(1, 0, 2)
             if out is None:

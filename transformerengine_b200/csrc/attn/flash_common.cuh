@@ -55,6 +55,7 @@ struct FlashParams {
   // sliding window: with `causal` set, key j is visible to query i when j <= i + causal_off (which
   // includes the right extent win_right) and, when has_lo, j >= i + lo_off
   int win_left, win_right, has_lo, lo_off;
+  int n_sink;        // keys j < n_sink are visible left of the window too
   int pair_balance;  // query-stationary kernels: a CTA takes 128-row tiles i and last - i (equal causal work)
 };
 
@@ -158,7 +159,13 @@ inline void set_mask_params(FlashParams& p, const FlashArgs& a) {
   p.has_lo = a.window_left >= 0 ? 1 : 0;
   p.win_left = a.window_left >= 0 ? a.window_left : 0;
   p.lo_off = base - p.win_left;
+  p.n_sink = p.has_lo && a.sink_tokens > 0 ? (a.sink_tokens < a.sk ? a.sink_tokens : a.sk) : 0;
 }
+
+// Mask variants compiled into the kernels: no lower bound, a sliding window, a window whose first keys stay visible.
+enum { kNoWindow = 0, kWindow = 1, kWindowSinks = 2 };
+
+inline int mask_variant(const FlashParams& p) { return !p.has_lo ? kNoWindow : (p.n_sink > 0 ? kWindowSinks : kWindow); }
 
 // 4-D tensor map over a [b, h, s, d] view; strides in elements, box = [rows x 64 elements]
 bool make_tensor_map_bhsd(CUtensorMap* map, const void* base, bool bf16, int b, int h, int s, long long sb,

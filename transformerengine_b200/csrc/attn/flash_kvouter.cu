@@ -28,7 +28,7 @@ struct KvCfg {
 };
 static_assert(KvCfg::kStageBytes % 1024 == 0, "ring stages must keep the swizzle alignment");
 
-template <bool BF, bool WIN>
+template <bool BF, int WIN>
 __global__ void __launch_bounds__(kThreads, 1)
 flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
@@ -60,7 +60,8 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   const int Gl = G / p.gsplit;  // query heads of this CTA
   const int kv0 = kb * 128;
   int nq = kv0 < p.sk ? (p.sq + 63) / 64 : 0;  // a key block past the sequence's end has no work
-  if (WIN && nq > 0) {  // sliding window: the last query that still sees the block's last key
+  // sliding window: the last query that still sees the block's last key (every later query sees the sinks)
+  if (WIN && nq > 0 && !(WIN == kWindowSinks && kv0 < p.n_sink)) {
     const int q_last = min(kv0 + 127, p.sk - 1) - p.lo_off;
     nq = q_last < 0 ? 0 : min(nq, q_last / 64 + 1);
   }
@@ -205,7 +206,7 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                              (WIN && qr + 63 > kv0 - p.lo_off);
       // key kv_row is visible to query q iff q >= q_min (and the key exists)
       const int q_min = kv_row < p.sk ? (p.causal ? kv_row - p.causal_off : 0) : 0x7fffffff;
-      const int q_max = WIN ? kv_row - p.lo_off : 0x7fffffff;
+      const int q_max = WIN && !(WIN == kWindowSinks && kv_row < p.n_sink) ? kv_row - p.lo_off : 0x7fffffff;
       uint32_t wp[16], wd[16];
       {
         uint32_t s[32], dp[32];
@@ -374,10 +375,12 @@ cudaError_t flash_bwd_dkdv(const FlashArgs& a, cudaStream_t stream) {
   if ((a.hq / a.hk) % p.gsplit != 0 || p.o_sg % 8 != 0) return cudaErrorInvalidValue;
   static bool attr_set = false;
   if (!attr_set) {
-    const void* fns[4] = {reinterpret_cast<const void*>(flash_kvouter_kernel<true, false>),
-                          reinterpret_cast<const void*>(flash_kvouter_kernel<false, false>),
-                          reinterpret_cast<const void*>(flash_kvouter_kernel<true, true>),
-                          reinterpret_cast<const void*>(flash_kvouter_kernel<false, true>)};
+    const void* fns[6] = {reinterpret_cast<const void*>(flash_kvouter_kernel<true, kNoWindow>),
+                          reinterpret_cast<const void*>(flash_kvouter_kernel<false, kNoWindow>),
+                          reinterpret_cast<const void*>(flash_kvouter_kernel<true, kWindow>),
+                          reinterpret_cast<const void*>(flash_kvouter_kernel<false, kWindow>),
+                          reinterpret_cast<const void*>(flash_kvouter_kernel<true, kWindowSinks>),
+                          reinterpret_cast<const void*>(flash_kvouter_kernel<false, kWindowSinks>)};
     for (const void* fn : fns) {
       cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
       if (e != cudaSuccess) return e;
@@ -385,11 +388,11 @@ cudaError_t flash_bwd_dkdv(const FlashArgs& a, cudaStream_t stream) {
     attr_set = true;
   }
   dim3 grid(a.hk * p.gsplit, (a.sk + 127) / 128, a.b);
-  const bool win = p.has_lo != 0;
-  if (bf && !win) flash_kvouter_kernel<true, false><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p);
-  else if (!win) flash_kvouter_kernel<false, false><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p);
-  else if (bf) flash_kvouter_kernel<true, true><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p);
-  else flash_kvouter_kernel<false, true><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p);
+  const auto go = [&](auto kernel) { kernel<<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p); };
+  const int win = mask_variant(p);
+  if (win == kNoWindow) bf ? go(flash_kvouter_kernel<true, kNoWindow>) : go(flash_kvouter_kernel<false, kNoWindow>);
+  else if (win == kWindow) bf ? go(flash_kvouter_kernel<true, kWindow>) : go(flash_kvouter_kernel<false, kWindow>);
+  else bf ? go(flash_kvouter_kernel<true, kWindowSinks>) : go(flash_kvouter_kernel<false, kWindowSinks>);
   return cudaGetLastError();
 }
 

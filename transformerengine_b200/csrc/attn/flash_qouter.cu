@@ -63,8 +63,9 @@ __device__ __forceinline__ int kv_blocks_of_tile(const FlashParams& p, int row0,
   return kv_end <= 0 ? 0 : (kv_end + bk - 1) / bk;
 }
 
-// WIN: sliding-window lower bound compiled in (kept out of the plain causal kernels)
-template <int MODE, bool BF, bool WIN>
+// WIN: mask variant compiled in (the lower bound is kept out of the plain causal kernels, the sinks out of the windowed
+// ones).  With sinks a CTA walks the key blocks that hold them first and then those of the window.
+template <int MODE, bool BF, int WIN>
 __global__ void __launch_bounds__(kThreads, 1)
 flash_qouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                     const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
@@ -112,6 +113,7 @@ flash_qouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   n[1] = kv_blocks_of_tile(p, qrow[1], BK);
   // sliding window: both tiles start at the first key block that the earlier tile can see
   int jbase = 0;
+  int nsb = 0;  // key blocks that hold the sinks, when they lie apart from the window's
   if (WIN) {
     int lo = 0x7fffffff;
     for (int t = 0; t < 2; ++t)
@@ -120,9 +122,15 @@ flash_qouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         lo = min(lo, first > 0 ? first / BK : 0);
       }
     jbase = lo == 0x7fffffff ? 0 : lo;
-    n[0] = n[0] > jbase ? n[0] - jbase : 0;
-    n[1] = n[1] > jbase ? n[1] - jbase : 0;
+    if (WIN == kWindowSinks) {
+      nsb = (min(p.n_sink, p.sk) + BK - 1) / BK;
+      if (nsb >= jbase) nsb = jbase = 0;  // no gap between the sinks and the window: one run of blocks
+    }
+    // (a tile may end before the window's first block, or among the sinks' blocks)
+    n[0] = min(n[0], nsb) + (n[0] > jbase ? n[0] - max(jbase, nsb) : 0);
+    n[1] = min(n[1], nsb) + (n[1] > jbase ? n[1] - max(jbase, nsb) : 0);
   }
+  const auto block_of = [&](int j) { return WIN == kWindowSinks && j < nsb ? j : jbase + j - nsb; };
   const int nmax = n[0] > n[1] ? n[0] : n[1];
 
   if (threadIdx.x == 0) {
@@ -171,11 +179,11 @@ flash_qouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         if (!mbar_wait(&k_empty[st], par)) { atomicCAS(p.status, 0, kFlashTimeoutProducer); break; }
         mbar_expect_tx(&k_full[st], C::kKvBytes);
         for (int pn = 0; pn < 2; ++pn)
-          tma_load_4d(smem + C::kOffK + st * C::kKvBytes + pn * C::kPanel, &tmap_k, &k_full[st], pn * 64, sv.k_off + (jbase + j) * BK, hk, sv.bt);
+          tma_load_4d(smem + C::kOffK + st * C::kKvBytes + pn * C::kPanel, &tmap_k, &k_full[st], pn * 64, sv.k_off + block_of(j) * BK, hk, sv.bt);
         if (!mbar_wait(&v_empty[st], par)) { atomicCAS(p.status, 0, kFlashTimeoutProducer); break; }
         mbar_expect_tx(&v_full[st], C::kKvBytes);
         for (int pn = 0; pn < 2; ++pn)
-          tma_load_4d(smem + C::kOffV + st * C::kKvBytes + pn * C::kPanel, &tmap_v, &v_full[st], pn * 64, sv.k_off + (jbase + j) * BK, hk, sv.bt);
+          tma_load_4d(smem + C::kOffV + st * C::kKvBytes + pn * C::kPanel, &tmap_v, &v_full[st], pn * 64, sv.k_off + block_of(j) * BK, hk, sv.bt);
       }
     }
   } else if (warp == 1) {
@@ -271,7 +279,7 @@ flash_qouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     }
   } else {
     const int t = (warp - 2) >> 3;
-    qouter_softmax_role<MODE, BF, C, WIN>(p, smem, s_full, p_ready, pv_done, xchg, tmem_base, warp, lane, qrow[t] - t * 128, h, b, n[t], t, jbase);
+    qouter_softmax_role<MODE, BF, C, WIN>(p, smem, s_full, p_ready, pv_done, xchg, tmem_base, warp, lane, qrow[t] - t * 128, h, b, n[t], t, jbase, nsb);
   }
 
   tc_fence_before();
@@ -342,10 +350,12 @@ static cudaError_t launch_qouter(const FlashArgs& a, cudaStream_t stream) {
   if (a.s_pad < a.sq) return cudaErrorInvalidValue;
   static bool attr_set = false;
   if (!attr_set) {
-    const void* fns[4] = {reinterpret_cast<const void*>(flash_qouter_kernel<MODE, true, false>),
-                          reinterpret_cast<const void*>(flash_qouter_kernel<MODE, false, false>),
-                          reinterpret_cast<const void*>(flash_qouter_kernel<MODE, true, true>),
-                          reinterpret_cast<const void*>(flash_qouter_kernel<MODE, false, true>)};
+    const void* fns[6] = {reinterpret_cast<const void*>(flash_qouter_kernel<MODE, true, kNoWindow>),
+                          reinterpret_cast<const void*>(flash_qouter_kernel<MODE, false, kNoWindow>),
+                          reinterpret_cast<const void*>(flash_qouter_kernel<MODE, true, kWindow>),
+                          reinterpret_cast<const void*>(flash_qouter_kernel<MODE, false, kWindow>),
+                          reinterpret_cast<const void*>(flash_qouter_kernel<MODE, true, kWindowSinks>),
+                          reinterpret_cast<const void*>(flash_qouter_kernel<MODE, false, kWindowSinks>)};
     for (const void* fn : fns) {
       cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
       if (e != cudaSuccess) return e;
@@ -358,11 +368,11 @@ static cudaError_t launch_qouter(const FlashArgs& a, cudaStream_t stream) {
     return e == nullptr || e[0] != '0';
   }();
   p.pair_balance = allow_pair && a.causal && a.window_left < 0 && static_cast<long long>(grid.x) * grid.y <= 148 ? 1 : 0;
-  const bool win = p.has_lo != 0;
-  if (bf && !win) flash_qouter_kernel<MODE, true, false><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p);
-  else if (!win) flash_qouter_kernel<MODE, false, false><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p);
-  else if (bf) flash_qouter_kernel<MODE, true, true><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p);
-  else flash_qouter_kernel<MODE, false, true><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p);
+  const auto go = [&](auto kernel) { kernel<<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p); };
+  const int win = mask_variant(p);
+  if (win == kNoWindow) bf ? go(flash_qouter_kernel<MODE, true, kNoWindow>) : go(flash_qouter_kernel<MODE, false, kNoWindow>);
+  else if (win == kWindow) bf ? go(flash_qouter_kernel<MODE, true, kWindow>) : go(flash_qouter_kernel<MODE, false, kWindow>);
+  else bf ? go(flash_qouter_kernel<MODE, true, kWindowSinks>) : go(flash_qouter_kernel<MODE, false, kWindowSinks>);
   return cudaGetLastError();
 }
 

@@ -1,0 +1,352 @@
+// 8-bit paged key/value cache: quantizing append, dequantizing gather, page copies.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "fp8_cache.cuh"
+#include "teb200/api.h"
+#include "teb200/kv_cache.h"
+
+namespace teb200 {
+namespace {
+
+using namespace kvc;
+
+// 8 consecutive values of a row as fp32
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(p + i);
+    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+  }
+}
+template <>
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+template <>
+__device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+// One warp per (sequence, 16-token block, head, K or V).  A lane owns 8 consecutive dims of the rows lane / (d / 8),
+// + 32 / (d / 8), ...; the block's largest finite magnitude sets the scale, and rows that were there before are rounded
+// again when it rises.  A power-of-two scale makes that second rounding exact except where a code becomes subnormal.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) append_kernel(const Fp8AppendArgs a) {
+  constexpr int kLanesPerRow = D / 8;
+  constexpr int kRows = 32 / kLanesPerRow;   // rows per pass
+  constexpr int kPasses = kKvBlock / kRows;
+  const int lane = threadIdx.x & 31;
+  const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);  // (head, K or V)
+  if (unit >= 2 * a.c.heads) return;
+  const int head = unit >> 1;
+  const bool is_v = unit & 1;
+  const int seq = blockIdx.z;
+  const int per = a.c.page_size / kKvBlock;
+  const int src0 = a.cu_new[seq];
+  const int n_new = a.cu_new[seq + 1] - src0;
+  const int len = a.c.kv_lens[seq];
+  const int old = len - n_new;
+  if (n_new <= 0) return;
+  if (old < 0 || src0 < 0 || src0 + n_new > a.t) {
+    if (lane == 0) atomicCAS(a.c.status, 0, kKvStatusPages);
+    return;
+  }
+  const T* src = static_cast<const T*>(is_v ? a.new_v : a.new_k) + head * (is_v ? a.v_sh : a.k_sh) +
+                 (lane % kLanesPerRow) * 8;
+  const long long st = is_v ? a.v_st : a.k_st;
+  for (int blk = old / kKvBlock + blockIdx.y; blk * kKvBlock < len; blk += gridDim.y) {
+    const int slot = blk / per;
+    const int page = slot < a.c.width ? a.c.table[static_cast<long long>(seq) * a.c.width + slot] : -1;
+    if (page < 0 || page >= a.c.pages) {
+      if (lane == 0) atomicCAS(a.c.status, 0, kKvStatusPages);
+      continue;
+    }
+    const long long idx = (static_cast<long long>(page) * a.c.heads + head) * per + blk % per;
+    uint8_t* codes = (is_v ? a.c.v : a.c.k) + idx * (kKvBlock * D) + lane * 8;
+    float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + idx;
+    const int first = max(old - blk * kKvBlock, 0);             // rows [first, end) are new
+    const int end = min(len - blk * kKvBlock, kKvBlock);
+    const T* rows = src + (src0 + blk * kKvBlock - old) * st;
+    float x[kPasses][8];
+    float top = 0.f;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int r = p * kRows + lane / kLanesPerRow;
+      if (r >= first && r < end) {
+        load8<T>(rows + r * st, x[p]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float m = fabsf(x[p][i]);
+          if (m < INFINITY) top = fmaxf(top, m);                // NaN and infinities do not set the scale
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float now = scale_for(top);
+    float was = now;
+    if (first > 0) {
+      was = *scale;
+      now = fmaxf(now, was);
+    }
+    __syncwarp();
+    const float inv = inverse_of_power(now);
+    const float again = was * inv;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int r = p * kRows + lane / kLanesPerRow;
+      uint2* dst = reinterpret_cast<uint2*>(codes + p * 256);
+      if (r >= first && r < end) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[p][i] *= inv;
+        *dst = make_uint2(to_e4m3x4(x[p][0], x[p][1], x[p][2], x[p][3]), to_e4m3x4(x[p][4], x[p][5], x[p][6], x[p][7]));
+      } else if (r < first && now != was) {
+        const uint2 old8 = *dst;
+        float y[8];
+        from_e4m3x4(old8.x, y);
+        from_e4m3x4(old8.y, y + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= again;
+        *dst = make_uint2(to_e4m3x4(y[0], y[1], y[2], y[3]), to_e4m3x4(y[4], y[5], y[6], y[7]));
+      }
+    }
+    if (lane == 0) *scale = now;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&y)[8]);
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float (&y)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(y[4], y[5], y[6], y[7]);
+}
+template <>
+__device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const float (&y)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack2<true>(y[0], y[1]), pack2<true>(y[2], y[3]), pack2<true>(y[4], y[5]),
+                                            pack2<true>(y[6], y[7]));
+}
+template <>
+__device__ __forceinline__ void store8<__half>(__half* p, const float (&y)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack2<false>(y[0], y[1]), pack2<false>(y[2], y[3]),
+                                            pack2<false>(y[4], y[5]), pack2<false>(y[6], y[7]));
+}
+
+// One warp per (sequence, 16-token block, head, K or V): codes * scale into a token-major buffer.  Blocks whose page is
+// not held, and the rows from a sequence's end to the next multiple of 128 (zero_to), become zeros.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
+  constexpr int kLanesPerRow = D / 8;
+  constexpr int kRows = 32 / kLanesPerRow;
+  constexpr int kPasses = kKvBlock / kRows;
+  const int lane = threadIdx.x & 31;
+  const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (unit >= 2 * a.c.heads) return;
+  const int head = unit >> 1;
+  const bool is_v = unit & 1;
+  const int seq = blockIdx.z;
+  const int per = a.c.page_size / kKvBlock;
+  const int len = a.c.kv_lens[seq];
+  const int off = a.off[seq];
+  const int stop = a.zero_to > 0 ? min((len + 127) / 128 * 128, a.zero_to) : len;
+  if (len < 0 || off < 0 || off + max(stop, len) > a.rows) {
+    if (lane == 0) atomicCAS(a.c.status, 0, kKvStatusPages);
+    return;
+  }
+  T* out = static_cast<T*>(is_v ? a.out_v : a.out_k) + static_cast<long long>(off) * a.c.heads * D + head * D +
+           (lane % kLanesPerRow) * 8;
+  for (int blk = blockIdx.y; blk * kKvBlock < stop; blk += gridDim.y) {
+    const int slot = blk / per;
+    int page = -1;
+    if (blk * kKvBlock < len) {
+      page = slot < a.c.width ? a.c.table[static_cast<long long>(seq) * a.c.width + slot] : a.c.pages;
+      if (page >= a.c.pages) {
+        if (lane == 0) atomicCAS(a.c.status, 0, kKvStatusPages);
+        page = -1;
+      }
+    }
+    const long long idx = page < 0 ? 0 : (static_cast<long long>(page) * a.c.heads + head) * per + blk % per;
+    const uint8_t* codes = (is_v ? a.c.v : a.c.k) + idx * (kKvBlock * D) + lane * 8;
+    const float scale = page < 0 ? 0.f : (is_v ? a.c.v_scale : a.c.k_scale)[idx];
+    uint2 w[kPasses];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = blk * kKvBlock + p * kRows + lane / kLanesPerRow;
+      w[p] = make_uint2(0u, 0u);
+      if (page >= 0 && row < len) w[p] = *reinterpret_cast<const uint2*>(codes + p * 256);
+    }
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = blk * kKvBlock + p * kRows + lane / kLanesPerRow;
+      if (row >= stop) continue;
+      float y[8];
+      from_e4m3x4(w[p].x, y);
+      from_e4m3x4(w[p].y, y + 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = w[p].x == 0u && w[p].y == 0u ? 0.f : y[i] * scale;
+      store8<T>(out + static_cast<long long>(row) * a.c.heads * D, y);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------- page copies
+constexpr int kCopyTensors = 128;
+constexpr int kCopyChunk = 16384;  // bytes per CTA step
+
+template <int PAIRS>
+struct CopyTable {
+  uint8_t* base[kCopyTensors];
+  long long page_bytes[kCopyTensors];
+  int chunk_start[kCopyTensors + 1];  // cumulative chunks (pairs * chunks per page)
+  int pairs, tensors;
+  int src[PAIRS], dst[PAIRS];
+};
+
+template <typename V>
+__device__ __forceinline__ void copy_range(uint8_t* dst, const uint8_t* src, int bytes) {
+  const int n = bytes / static_cast<int>(sizeof(V));
+  const V* s = reinterpret_cast<const V*>(src);
+  V* d = reinterpret_cast<V*>(dst);
+  int i = threadIdx.x;
+  for (; i + 3 * static_cast<int>(blockDim.x) < n; i += 4 * blockDim.x) {
+    V v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = s[i + u * blockDim.x];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) d[i + u * blockDim.x] = v[u];
+  }
+  for (; i < n; i += blockDim.x) d[i] = s[i];
+}
+
+template <int PAIRS>
+__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyTable<PAIRS> t) {
+  const int total = t.chunk_start[t.tensors];
+  for (int c = blockIdx.x; c < total; c += gridDim.x) {
+    int lo = 0, hi = t.tensors - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (t.chunk_start[mid] <= c) lo = mid; else hi = mid - 1;
+    }
+    const long long pb = t.page_bytes[lo];
+    const int per = static_cast<int>((pb + kCopyChunk - 1) / kCopyChunk);
+    const int rel = c - t.chunk_start[lo];
+    const int pair = rel / per;
+    const long long at = static_cast<long long>(rel % per) * kCopyChunk;
+    const int bytes = static_cast<int>(pb - at < kCopyChunk ? pb - at : kCopyChunk);
+    const uint8_t* s = t.base[lo] + t.src[pair] * pb + at;
+    uint8_t* d = t.base[lo] + t.dst[pair] * pb + at;
+    const uint64_t align = reinterpret_cast<uint64_t>(t.base[lo]) | static_cast<uint64_t>(pb);
+    if (align % 16 == 0) copy_range<uint4>(d, s, bytes);
+    else if (align % 4 == 0) copy_range<uint32_t>(d, s, bytes);
+    else copy_range<uint8_t>(d, s, bytes);
+  }
+}
+
+template <int PAIRS>
+cudaError_t launch_copy(const PageCopyTensor* tensors, int num_tensors, const int* src, const int* dst, int pairs,
+                        cudaStream_t stream) {
+  CopyTable<PAIRS> t;
+  t.pairs = pairs;
+  t.tensors = num_tensors;
+  long long chunks = 0;
+  for (int i = 0; i < num_tensors; ++i) {
+    t.base[i] = static_cast<uint8_t*>(tensors[i].base);
+    t.page_bytes[i] = tensors[i].page_bytes;
+    t.chunk_start[i] = static_cast<int>(chunks);
+    chunks += (tensors[i].page_bytes + kCopyChunk - 1) / kCopyChunk * pairs;
+    if (chunks > 0x7fffffff) return cudaErrorInvalidValue;
+  }
+  t.chunk_start[num_tensors] = static_cast<int>(chunks);
+  for (int i = 0; i < pairs; ++i) {
+    t.src[i] = src[i];
+    t.dst[i] = dst[i];
+  }
+  if (chunks == 0) return cudaSuccess;
+  const int grid = static_cast<int>(chunks < 148 * 8 ? chunks : 148 * 8);
+  copy_pages_kernel<PAIRS><<<grid, 256, 0, stream>>>(t);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t append_d(const Fp8AppendArgs& a, dim3 grid, cudaStream_t s) {
+  if (a.c.d == 64) append_kernel<T, 64><<<grid, 128, 0, s>>>(a);
+  else if (a.c.d == 128) append_kernel<T, 128><<<grid, 128, 0, s>>>(a);
+  else if (a.c.d == 256) append_kernel<T, 256><<<grid, 128, 0, s>>>(a);
+  else return cudaErrorInvalidValue;
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t gather_d(const Fp8GatherArgs& a, dim3 grid, cudaStream_t s) {
+  if (a.c.d == 64) gather_kernel<T, 64><<<grid, 128, 0, s>>>(a);
+  else if (a.c.d == 128) gather_kernel<T, 128><<<grid, 128, 0, s>>>(a);
+  else if (a.c.d == 256) gather_kernel<T, 256><<<grid, 128, 0, s>>>(a);
+  else return cudaErrorInvalidValue;
+  return cudaGetLastError();
+}
+
+bool view_ok(const Fp8CacheView& c) {
+  return c.pages > 0 && c.heads > 0 && c.page_size >= kKvBlock && c.page_size % kKvBlock == 0 && c.n <= 65535 &&
+         c.width > 0;
+}
+
+}  // namespace
+
+cudaError_t fp8_cache_append(const Fp8AppendArgs& a, cudaStream_t s) {
+  if (!view_ok(a.c)) return cudaErrorInvalidValue;
+  if (a.c.n == 0 || a.t == 0) return cudaSuccess;
+  int blocks = (a.max_new + kKvBlock - 2) / kKvBlock + 1;  // a run may start on a block's last row
+  if (blocks > 65535) blocks = 65535;
+  const dim3 grid((2 * a.c.heads + 3) / 4, blocks, a.c.n);
+  if (a.dtype == kFloat32) return append_d<float>(a, grid, s);
+  if (a.dtype == kFloat16) return append_d<__half>(a, grid, s);
+  if (a.dtype == kBFloat16) return append_d<__nv_bfloat16>(a, grid, s);
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t fp8_cache_gather(const Fp8GatherArgs& a, cudaStream_t s) {
+  if (!view_ok(a.c)) return cudaErrorInvalidValue;
+  if (a.c.n == 0 || a.rows == 0) return cudaSuccess;
+  int blocks = (a.max_kv + 127) / 128 * 8;
+  blocks = blocks < 1 ? 1 : (blocks > 65535 ? 65535 : blocks);
+  const dim3 grid((2 * a.c.heads + 3) / 4, blocks, a.c.n);
+  if (a.dtype == kFloat32) return gather_d<float>(a, grid, s);
+  if (a.dtype == kFloat16) return gather_d<__half>(a, grid, s);
+  if (a.dtype == kBFloat16) return gather_d<__nv_bfloat16>(a, grid, s);
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t copy_pages(const PageCopyTensor* tensors, int num_tensors, const int* src, const int* dst, int pairs,
+                       cudaStream_t stream) {
+  // the table travels in the launch parameters: a small one for a fork, a large one for a compaction
+  for (int t0 = 0; t0 < num_tensors; t0 += kCopyTensors) {
+    const int nt = num_tensors - t0 < kCopyTensors ? num_tensors - t0 : kCopyTensors;
+    for (int p0 = 0; p0 < pairs; p0 += 1024) {
+      const int np = pairs - p0 < 1024 ? pairs - p0 : 1024;
+      const cudaError_t e = np <= 64 ? launch_copy<64>(tensors + t0, nt, src + p0, dst + p0, np, stream)
+                                     : launch_copy<1024>(tensors + t0, nt, src + p0, dst + p0, np, stream);
+      if (e != cudaSuccess) return e;
+    }
+  }
+  return cudaSuccess;
+}
+
+}  // namespace teb200

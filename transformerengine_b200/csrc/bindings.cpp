@@ -455,6 +455,7 @@ void rope(const at::Tensor& x, at::Tensor& out, const at::Tensor& freqs, int64_t
 }  // namespace
 
 void register_extra(py::module_& m);  // bindings of kernels added in other translation units
+void register_kv(py::module_& m);     // bindings_kv.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("status", teb200::traced("teb200.status", &status));
@@ -483,4 +484,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("start_positions"), py::arg("qkv_mode") = 0, py::arg("q_per_group") = 0, py::arg("hq") = 0,
         py::arg("hk") = 0, py::arg("freqs_k") = py::none());
   register_extra(m);
+  register_kv(m);
 }

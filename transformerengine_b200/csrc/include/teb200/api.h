@@ -99,6 +99,8 @@ struct FlashArgs {
   // Sliding window: query i (diagonal-aligned like the causal mask) sees keys in
   // [i - window_left, i + window_right]; -1 = unbounded.  causal forces window_right = 0.
   int window_left = -1, window_right = -1;
+  // Left of the window the first sink_tokens keys stay visible (0: none; only read with window_left >= 0).
+  int sink_tokens = 0;
 };
 cudaError_t flash_fwd(const FlashArgs& args, cudaStream_t stream);
 cudaError_t flash_delta(const FlashArgs& args, cudaStream_t stream);     // delta = rowsum(dO * O)

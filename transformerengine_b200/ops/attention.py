@@ -18,8 +18,9 @@ import torch
 from . import _ext
 
 
-def _build_mask(sq, sk, device, causal, window, bottom_right=True):
-    """True = masked out.  ``window`` = (left, right) with -1 meaning unbounded."""
+def _build_mask(sq, sk, device, causal, window, bottom_right=True, sink_tokens=0):
+    """True = masked out.  ``window`` = (left, right) with -1 meaning unbounded; the first ``sink_tokens`` keys stay
+    visible left of the window."""
     if not causal and (window is None or (window[0] < 0 and window[1] < 0)):
         return None
     qi = torch.arange(sq, device=device)[:, None]
@@ -32,13 +33,13 @@ def _build_mask(sq, sk, device, causal, window, bottom_right=True):
     if right >= 0:
         m |= rel > right
     if left >= 0:
-        m |= rel < -left
+        m |= (rel < -left) & (ki >= sink_tokens)
     return m
 
 
 def attention_ref(q, k, v, *, scale=None, causal=False, window=None, attn_mask=None, bias=None, dropout_p=0.0,
                   softmax_type="vanilla", sink=None, bottom_right=True, generator=None, return_lse=False,
-                  score_mod=None, score_mod_tensors=None):
+                  score_mod=None, score_mod_tensors=None, sink_tokens=0):
     """fp32 attention on ``[b, h, s, d]`` tensors; k/v may have fewer heads (GQA).
     ``score_mod(score, tensors) -> score`` edits the scaled scores ``[b, h, sq, sk]`` before masking."""
     b, hq, sq, d = q.shape
@@ -54,7 +55,7 @@ def attention_ref(q, k, v, *, scale=None, causal=False, window=None, attn_mask=N
         s = s + bias.float()
     if score_mod is not None:
         s = score_mod(s, score_mod_tensors or {})
-    m = _build_mask(sq, sk, q.device, causal, window, bottom_right)
+    m = _build_mask(sq, sk, q.device, causal, window, bottom_right, sink_tokens)
     if m is not None:
         s = s.masked_fill(m, float("-inf"))
     if attn_mask is not None:
@@ -78,7 +79,7 @@ def attention_ref(q, k, v, *, scale=None, causal=False, window=None, attn_mask=N
 
 @torch.no_grad()
 def max_attention_logit(q, k, *, scale=None, causal=False, window=None, attn_mask=None, bias=None,
-                        bottom_right=True, chunk_bytes: int = 256 << 20) -> torch.Tensor:
+                        bottom_right=True, chunk_bytes: int = 256 << 20, sink_tokens: int = 0) -> torch.Tensor:
     """Per-head maximum of the scaled, biased and masked attention scores of ``[b, h, s, d]`` tensors (fp32 ``[h]``;
     the quantity "QK-clip" optimizers watch).  A pass of its own over Q K^T in blocks of query rows, so that no
     ``s x s`` score tensor is kept.  (Reference: ``return_max_logit`` of
@@ -90,7 +91,7 @@ def max_attention_logit(q, k, *, scale=None, causal=False, window=None, attn_mas
     if hk != hq:
         kf = kf.repeat_interleave(hq // hk, dim=1)
     kt = kf.transpose(-1, -2)
-    m = _build_mask(sq, sk, q.device, causal, window, bottom_right)
+    m = _build_mask(sq, sk, q.device, causal, window, bottom_right, sink_tokens)
     rows = max(1, min(sq, chunk_bytes // max(4 * b * hq * sk, 1)))
     best = torch.full((hq,), float("-inf"), dtype=torch.float32, device=q.device)
     for r0 in range(0, sq, rows):
@@ -119,14 +120,20 @@ _USE_LIBRARY_SDPA = _get_config().attention_backend != "reference"
 
 def attention(q, k, v, *, scale=None, causal=False, window=None, attn_mask=None, bias=None, dropout_p=0.0,
               softmax_type="vanilla", sink=None, bottom_right=True, out_format="bhsd", score_mod=None,
-              score_mod_tensors=None):
+              score_mod_tensors=None, sink_tokens=0):
     """Differentiable attention on ``[b, h, s, d]``; ``out_format`` names the memory layout of the
     returned ``[b, h, s, d]`` view ("bhsd", "sbhd" or "bshd") when the fused kernel runs.
+
+    ``sink_tokens``: the first keys that stay visible to every query (up to the causal diagonal) although they lie left
+    of the sliding window; without a left side of ``window`` it changes nothing.  (``sink`` is another thing: the extra
+    logit of ``softmax_type="learnable"``.)
 
     On CUDA the fused flash kernel of this library handles the common case
     (16-bit, no bias / arbitrary mask / dropout, head dim 64 or 128); everything
     else runs the reference math, which autograd differentiates.
     """
+    if sink_tokens < 0:
+        raise ValueError("sink_tokens must not be negative")
     no_window = window is None or (window[0] < 0 and (window[1] < 0 or (causal and window[1] == 0)))
     plain = attn_mask is None and bias is None and dropout_p == 0.0 and softmax_type == "vanilla" and \
         score_mod is None
@@ -135,13 +142,13 @@ def attention(q, k, v, *, scale=None, causal=False, window=None, attn_mask=None,
 
         if _USE_OWN_FLASH and flash.supported(q, k, v, causal):
             return flash.flash_attention(q, k, v, scale, causal, bottom_right, out_format,
-                                         None if no_window else window)
+                                         None if no_window else window, sink_tokens)
         if _USE_LIBRARY_SDPA and no_window and (not causal or q.shape[2] == k.shape[2] or not bottom_right):
             return torch.nn.functional.scaled_dot_product_attention(
                 q, k, v, is_causal=causal, scale=scale, enable_gqa=q.shape[1] != k.shape[1])
     return attention_ref(q, k, v, scale=scale, causal=causal, window=window, attn_mask=attn_mask, bias=bias,
                          dropout_p=dropout_p, softmax_type=softmax_type, sink=sink, bottom_right=bottom_right,
-                         score_mod=score_mod, score_mod_tensors=score_mod_tensors)
+                         score_mod=score_mod, score_mod_tensors=score_mod_tensors, sink_tokens=sink_tokens)
 
 
 def merge_attention_states(o1, lse1, o2, lse2) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -43,7 +43,7 @@ def _empty_out(q: torch.Tensor, out_format: str) -> torch.Tensor:
 
 class _FlashFunc(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, scale, causal, bottom_right, out_format, window):  # type: ignore[override]
+    def forward(ctx, q, k, v, scale, causal, bottom_right, out_format, window, sink_tokens):  # type: ignore[override]
         C_ = _ext.get()
         q, k, v = _prep(q), _prep(k), _prep(v)
         b, h, sq, d = q.shape
@@ -53,32 +53,40 @@ class _FlashFunc(torch.autograd.Function):
         sc = float(scale) if scale is not None else d ** -0.5
         wl, wr = (-1, -1) if window is None else (int(window[0]), int(window[1]))
         C_.flash_fwd(q, k, v, out, lse, sc, bool(causal), bool(bottom_right), C_.status(q.device.index),
-                     window_left=wl, window_right=wr)
+                     window_left=wl, window_right=wr, sink_tokens=sink_tokens)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.cfg = (sc, bool(causal), bool(bottom_right), wl, wr)
+        ctx.cfg = (sc, bool(causal), bool(bottom_right), wl, wr, sink_tokens)
         return out
 
     @staticmethod
     def backward(ctx, dout):  # type: ignore[override]
         C_ = _ext.get()
         q, k, v, out, lse = ctx.saved_tensors
-        sc, causal, bottom_right, wl, wr = ctx.cfg
+        sc, causal, bottom_right, wl, wr, sink_tokens = ctx.cfg
         dout = _prep(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         if dk.stride() != dv.stride():
             dv = torch.empty_strided(dk.shape, dk.stride(), dtype=dk.dtype, device=dk.device)
         delta = torch.empty_like(lse)
         C_.flash_bwd(dout, q, k, v, out, lse, delta, dq, dk, dv, sc, causal, bottom_right,
-                     C_.status(q.device.index), window_left=wl, window_right=wr)
-        return dq, dk, dv, None, None, None, None, None
+                     C_.status(q.device.index), window_left=wl, window_right=wr, sink_tokens=sink_tokens)
+        return dq, dk, dv, None, None, None, None, None, None
 
 
-def flash_attention(q, k, v, scale, causal, bottom_right=True, out_format: str = "bhsd", window=None):
+def _sinks(window, sink_tokens: int, sk: int) -> int:
+    """Sinks matter only left of a window, and no further than the keys reach (fits the kernels' 32-bit fields)."""
+    return 0 if window is None or window[0] < 0 else min(int(sink_tokens), sk)
+
+
+def flash_attention(q, k, v, scale, causal, bottom_right=True, out_format: str = "bhsd", window=None,
+                    sink_tokens: int = 0):
     """``window = (left, right)``: query i sees keys [i - left, i + right] around the (bottom-right or
-    top-left aligned) diagonal, -1 = unbounded; ``causal`` forces right = 0."""
+    top-left aligned) diagonal, -1 = unbounded; ``causal`` forces right = 0.  The first ``sink_tokens`` keys stay visible
+    left of the window."""
     if window is not None and window[0] < 0 and window[1] < 0:
         window = None
-    return _FlashFunc.apply(q, k, v, scale, causal, bottom_right, out_format, window)
+    return _FlashFunc.apply(q, k, v, scale, causal, bottom_right, out_format, window,
+                            _sinks(window, sink_tokens, k.shape[2]))
 
 
 def flash_forward_lse(q, k, v, scale, causal, bottom_right=True):
@@ -116,7 +124,8 @@ def _thd_view(t: torch.Tensor) -> torch.Tensor:
 
 class _FlashVarlenFunc(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, cu_q, cu_k, off_q, off_k, max_sq, max_sk, scale, causal, bottom_right, window):  # type: ignore[override]
+    def forward(ctx, q, k, v, cu_q, cu_k, off_q, off_k, max_sq, max_sk, scale, causal, bottom_right, window,
+                sink_tokens):  # type: ignore[override]
         C_ = _ext.get()
         tq, hq, d = q.shape
         nseq = cu_q.numel() - 1
@@ -128,29 +137,41 @@ class _FlashVarlenFunc(torch.autograd.Function):
         wl, wr = (-1, -1) if window is None else (int(window[0]), int(window[1]))
         C_.flash_fwd_varlen(qv, kv, vv, _thd_view(out), lse, cu_q, cu_k, off_q, off_k, max_sq, max_sk, sc,
                             bool(causal), bool(bottom_right), C_.status(q.device.index), window_left=wl,
-                            window_right=wr)
+                            window_right=wr, sink_tokens=sink_tokens)
         ctx.save_for_backward(qv, kv, vv, out, lse, cu_q, cu_k, off_q, off_k)
-        ctx.cfg = (sc, bool(causal), bool(bottom_right), max_sq, max_sk, wl, wr)
+        ctx.cfg = (sc, bool(causal), bool(bottom_right), max_sq, max_sk, wl, wr, sink_tokens)
         return out
 
     @staticmethod
     def backward(ctx, dout):  # type: ignore[override]
         C_ = _ext.get()
         qv, kv, vv, out, lse, cu_q, cu_k, off_q, off_k = ctx.saved_tensors
-        sc, causal, bottom_right, max_sq, max_sk, wl, wr = ctx.cfg
+        sc, causal, bottom_right, max_sq, max_sk, wl, wr, sink_tokens = ctx.cfg
         dq = torch.zeros(qv.shape[2], qv.shape[1], 128, dtype=qv.dtype, device=qv.device)
         dk = torch.zeros(kv.shape[2], kv.shape[1], 128, dtype=qv.dtype, device=qv.device)
         dv = torch.zeros_like(dk)
         delta = torch.empty_like(lse)
         C_.flash_bwd_varlen(_thd_view(dout), qv, kv, vv, _thd_view(out), lse, delta, _thd_view(dq), _thd_view(dk),
                             _thd_view(dv), cu_q, cu_k, off_q, off_k, max_sq, max_sk, sc, causal, bottom_right,
-                            C_.status(qv.device.index), window_left=wl, window_right=wr)
-        return (dq, dk, dv) + (None,) * 10
+                            C_.status(qv.device.index), window_left=wl, window_right=wr, sink_tokens=sink_tokens)
+        return (dq, dk, dv) + (None,) * 11
+
+
+def flash_varlen_forward(q, k, v, cu_q, cu_k, off_q, off_k, max_sq, max_sk, scale, causal, window_left, sink_tokens):
+    """Forward only, bottom-right aligned: the attention of prompt chunks over an expanded key/value cache.  Rows of ``q``
+    outside every sequence give zeros."""
+    C_ = _ext.get()
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(cu_q.numel() - 1, q.shape[1], (max_sq + 127) // 128 * 128, dtype=torch.float32, device=q.device)
+    C_.flash_fwd_varlen(_thd_view(q), _thd_view(k), _thd_view(v), _thd_view(out), lse, cu_q, cu_k, off_q, off_k, max_sq,
+                        max_sk, scale, bool(causal), True, C_.status(q.device.index), window_left=window_left,
+                        window_right=-1, sink_tokens=_sinks((window_left, -1), sink_tokens, max_sk))
+    return out
 
 
 def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_kv, scale=None, causal=False, bottom_right=True,
                            max_seqlen_q=None, max_seqlen_kv=None, cu_seqlens_q_padded=None,
-                           cu_seqlens_kv_padded=None, window=None):
+                           cu_seqlens_kv_padded=None, window=None, sink_tokens: int = 0):
     """Attention over packed sequences.  ``q`` is ``[tq, hq, 128]``, ``k`` / ``v`` ``[tk, hk, 128]``;
     sequence i owns ``cu_seqlens[i+1] - cu_seqlens[i]`` tokens starting at ``cu_seqlens_padded[i]``
     (``cu_seqlens[i]`` when no padded offsets are given).  Returns ``[tq, hq, 128]``."""
@@ -167,4 +188,4 @@ def flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_kv, scale=None, cau
     if window is not None and window[0] < 0 and (window[1] < 0 or (causal and window[1] == 0)):
         window = None
     return _FlashVarlenFunc.apply(q, k, v, cu_q, cu_k, off_q, off_k, int(max_seqlen_q), int(max_seqlen_kv), scale,
-                                  causal, bottom_right, window)
+                                  causal, bottom_right, window, _sinks(window, sink_tokens, int(max_seqlen_kv)))
