@@ -441,3 +441,90 @@ def test_zero_sinks_are_the_plain_window():
     assert torch.equal(a, te.functional.attention(q, k, v, causal=True, window=(70, 0), sink_tokens=0))
     b = te.functional.attention(q, k, v, causal=True)
     assert torch.equal(b, te.functional.attention(q, k, v, causal=True, sink_tokens=9))      # no window: nothing to see past
+
+
+# ------------------------------------------------------------------------------------------------ as a model uses them
+from collections import OrderedDict  # noqa: E402
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_model_on_the_8_bit_cache_with_forks_drafts_and_compaction(head_dim):
+    """Prompt, forks, single tokens, drafts cut back, compaction, pages out of the window reused: the logits stay by the
+    full pass's, and by those of the CPU path on the same codes' rounding."""
+    from transformerengine_b200.models.mistral import MistralConfig, MistralModel
+    torch.manual_seed(3)
+    cfg = MistralConfig.tiny(hidden_size=512, num_heads=512 // head_dim, num_kv_heads=2, head_dim=head_dim, sliding_window=100, sink_tokens=5)
+    model = MistralModel(cfg).cuda().eval()
+    tokens = torch.randint(0, cfg.vocab_size, (2, 320), device="cuda")
+    with torch.no_grad():
+        full = model(tokens).transpose(0, 1).float()
+        params = model.make_inference_params(4, 400, is_paged=True, page_size=32, total_num_pages=64, cache_dtype=torch.float8_e4m3fn)
+        m = params.cache_manager
+        at = 300
+        params.pre_step(OrderedDict([(0, at), (1, at)]))
+        got = [model(tokens[:, :at], inference_params=params).transpose(0, 1).float()]
+        rows = []
+        for n, junk in ((1, 0), (1, 0), (2, 3), (1, 0), (5, 2)):
+            params.fork_sequence(1, 9 + at)                                # a fork that is gone with the next step
+            params.pre_step(OrderedDict([(0, n + junk), (1, n + junk), (9 + at, 1)]))
+            pad = torch.zeros(1, n + junk, dtype=torch.long, device="cuda")
+            step = torch.cat([tokens[:, at:at + n], torch.randint(0, cfg.vocab_size, (2, junk), device="cuda")], 1)
+            y = model(torch.cat([step, pad]), inference_params=params).transpose(0, 1).float()
+            rows.append(y[:2, :n])
+            at += n
+            for i in (0, 1):
+                params.truncate_sequence(i, at)
+            if n == 2:
+                params.compact()
+        got = torch.cat(got + rows, 1)
+    te.check_status()
+    assert m.page_table[0][0] >= 0 and m.page_table[0][2] == -1
+    for i in (0, 1):
+        # keys and values off by up to 2^-4 each, in two layers
+        assert (got[i] - full[i, :at]).norm() / full[i, :at].norm() < 2.0 ** -3
+    out = model.generate(tokens[:, :50], 30, is_paged=True, page_size=32, total_num_pages=16, cache_dtype=torch.float8_e4m3fn)
+    assert out.shape == (2, 80)
+    te.check_status()
+
+
+def test_16_bit_pages_fork_and_copy_on_the_gpu():
+    m = te.PagedKVCacheManager(8, 16, 2, 64, torch.bfloat16, 4, 128, device="cuda")
+    x = torch.randn(22, 2, 64, device="cuda", dtype=torch.bfloat16)
+    m.pre_step(OrderedDict([(0, 20)]))
+    m.step(1, x[:20], x[:20] + 1, [0, 20])
+    m.post_step()
+    m.fork_sequence(0, 1)
+    m.pre_step(OrderedDict([(0, 1), (1, 1)]))
+    k, v, _ = m.step(1, x[20:], x[20:] + 1, [0, 1, 2])
+    assert torch.equal(k, torch.cat([x[:21], x[:20], x[21:]])) and torch.equal(v, k + 1)
+    te.check_status()
+
+
+def test_forward_and_backward_with_sinks_in_a_captured_graph():
+    """Replays give the eager results.  The captured leaves are their own (views of the same memory): autograd ties a
+    leaf's gradient node to the stream of the eager graph that made it, so PyTorch itself cannot capture a backward pass
+    of leaves whose eager graph is still alive."""
+    g = torch.Generator().manual_seed(17)
+    q, k, v = (torch.randn(1, h, 300, 128, generator=g).to(torch.bfloat16).cuda().requires_grad_() for h in (4, 2, 2))
+    do = torch.randn(1, 4, 300, 128, generator=g).to(torch.bfloat16).cuda()
+
+    def both():
+        own = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = te.functional.attention(*own, causal=True, window=(50, 0), sink_tokens=4)
+        return (o.detach(), *torch.autograd.grad(o, own, do))
+
+    kept = te.functional.attention(q, k, v, causal=True, window=(50, 0), sink_tokens=4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for t in got:
+        t.zero_()
+    graph.replay()
+    want = (kept.detach(), *torch.autograd.grad(kept, (q, k, v), do))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    te.check_status()

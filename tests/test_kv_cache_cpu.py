@@ -208,3 +208,185 @@ def test_sink_tokens_refuses_a_negative_count():
     q = torch.zeros(1, 1, 2, 8)
     with pytest.raises(ValueError, match="negative"):
         te.functional.attention(q, q, q, causal=True, window=(1, 0), sink_tokens=-1)
+
+
+# ----------------------------------------------------------------------------------------- managers, modules, generation
+from collections import OrderedDict  # noqa: E402
+
+
+def _paged(fp8, **kw):
+    d = dict(total_num_pages=8, page_size=16, num_heads_kv=1, head_dim_k=8, dtype=torch.float32, max_batch_size=4,
+             max_sequence_length=128, device="cpu")
+    d.update(kw)
+    return (te.FP8PagedKVCacheManager if fp8 else te.PagedKVCacheManager)(**d)
+
+
+def _tokens(m, x):
+    """One step of every sequence in m.step_dict: keys x, values -x."""
+    cu = [0]
+    for n in m.step_dict.values():
+        cu.append(cu[-1] + n)
+    k, v, lens = m.step(1, x, -x, cu)
+    m.post_step()
+    return k, lens
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_forked_sequences_share_pages_until_one_writes(fp8):
+    m = _paged(fp8)
+    g = torch.Generator().manual_seed(3)
+    # powers of two are exact in 8 bits
+    x = torch.exp2(torch.randint(-3, 4, (40, 1, 8), generator=g).float())
+    m.pre_step(OrderedDict([(0, 20)]))
+    _tokens(m, x[:20])
+    m.fork_sequence(0, 1)
+    m.fork_sequence(0, 2)
+    assert m.page_table[1] == m.page_table[0] and len(m.free_pages) == 6
+    m.pre_step(OrderedDict([(0, 1), (1, 1), (2, 0)]))
+    assert m.page_table[0][0] == m.page_table[1][0] == m.page_table[2][0]
+    assert len({m.page_table[i][1] for i in range(3)}) == 3 and len(m.free_pages) == 4
+    k, lens = _tokens(m, x[20:22])
+    assert lens == [21, 21, 20]
+    assert torch.equal(k[:20], x[:20]) and torch.equal(k[20], x[20]) and torch.equal(k[21:41], x[:20]) and torch.equal(k[41], x[21])
+    assert torch.equal(k[42:], x[:20])
+    m.truncate_sequence(1, 16)                        # its copy of the second page goes back
+    assert len(m.free_pages) == 5 and m.lengths[1] == 16
+    m.deallocate_sequence(0)
+    assert len(m.free_pages) == 6                     # the first page has two owners left
+    moved = m.compact()
+    used = {p for t in m.page_table.values() for p in t}
+    assert used == set(range(len(used))) and sorted(m.free_pages + list(used)) == list(range(8)) and moved <= 2
+    m.pre_step(OrderedDict([(1, 2), (2, 1)]))
+    k, _ = _tokens(m, x[22:25])
+    assert torch.equal(k[:16], x[:16]) and torch.equal(k[16:18], x[22:24]) and torch.equal(k[18:38], x[:20]) and torch.equal(k[38], x[24])
+    m.pre_step(OrderedDict())
+    assert len(m.free_pages) == 8 and not m.page_refs
+
+
+def test_manager_refusals():
+    m = _paged(True)
+    m.pre_step(OrderedDict([(0, 20)]))
+    m.post_step()
+    for call, what in ((lambda: m.fork_sequence(5, 6), "unknown"), (lambda: m.fork_sequence(0, 0), "exists"),
+                       (lambda: m.truncate_sequence(0, 21), "cannot cut"), (lambda: m.truncate_sequence(9, 0), "unknown")):
+        with pytest.raises(ValueError, match=what):
+            call()
+    m.fork_sequence(0, 1), m.fork_sequence(0, 2), m.fork_sequence(0, 3)
+    with pytest.raises(ValueError, match="max_batch_size"):
+        m.fork_sequence(0, 4)
+    with pytest.raises(AssertionError, match="out of pages"):
+        m.pre_step(OrderedDict([(0, 1), (1, 1), (2, 90), (3, 0)]))
+    with pytest.raises(ValueError, match="multiple of 16"):
+        _paged(True, page_size=8)
+    kw = dict(num_heads_kv=1, head_dim_k=8, dtype=torch.float32, device="cpu")
+    with pytest.raises(ValueError, match="is paged"):
+        te.InferenceParams(2, 32, cache_dtype=torch.float8_e4m3fn, **kw)
+    with pytest.raises(ValueError, match="cache_dtype"):
+        te.InferenceParams(2, 32, cache_dtype=torch.int8, **kw)
+    with pytest.raises(ValueError, match="8-bit cache"):
+        te.InferenceParams(2, 32, window_size=4, **kw)
+
+
+def test_pages_out_of_the_window_return_to_the_pool():
+    m = _paged(True, window_size=20, sink_tokens=3, total_num_pages=5)
+    g = torch.Generator().manual_seed(4)
+    x = torch.exp2(torch.randint(-3, 4, (100, 1, 8), generator=g).float())
+    q = torch.randn(100, 2, 8, generator=g)
+    full = kc.FP8KVCache.allocate(7, 1, 16, 8, device="cpu")
+    kc.append(full, x, -x, _i32([list(range(7))]), _i32([0, 100]), _i32([100]))
+    done = 0
+    for n in [30] + [10] * 7:
+        m.pre_step(OrderedDict([(0, n)]))
+        o = m.attend(1, q[done:done + n], x[done:done + n], -x[done:done + n], scale=1.0, causal=True, window=(20, 0), sink_tokens=3)
+        m.post_step()
+        done += n
+        want = kc.attend(q[done - n:done], full, _i32([list(range(7))]), _i32([0, n]), _i32([done]), max_q=n, max_kv=done, scale=1.0,
+                         window=(20, 0), sink_tokens=3)
+        torch.testing.assert_close(o, want, rtol=0, atol=0)
+    assert m.page_table[0][0] >= 0 and m.page_table[0][1] == -1 and len(m.page_table[0]) == 7
+    with pytest.raises(ValueError, match="given back"):
+        m.truncate_sequence(0, 40)
+    m.truncate_sequence(0, 97)
+    with pytest.raises(ValueError, match="keeps a window"):
+        m.attend(1, q[:1], x[:1], x[:1], scale=1.0, causal=True, window=(21, 0), sink_tokens=3)
+    with pytest.raises(ValueError, match="keeps a window"):
+        m.attend(1, q[:1], x[:1], x[:1], scale=1.0, causal=True, window=None, sink_tokens=3)
+
+
+@pytest.mark.parametrize("fmt", ["bshd", "sbhd"])
+@pytest.mark.parametrize("window,sinks", [(None, 0), ((4, 0), 2)])
+def test_incremental_attention_on_the_8_bit_cache(fmt, window, sinks):
+    """Step by step equals one pass, up to the rounding of keys and values (half a step of e4m3 and a requantization)."""
+    torch.manual_seed(0)
+    b, h, hk, d, total = 2, 4, 2, 16, 20
+    mha = te.MultiheadAttention(h * d, h, num_gqa_groups=hk, attention_dropout=0.0, attn_mask_type="causal", qkv_format=fmt, bias=False,
+                                params_dtype=torch.float32, device="cpu", window_size=window, sink_tokens=sinks).eval()
+    rope = te.RotaryPositionEmbedding(d)(64)          # the cache's length: padding has positions too
+    x = torch.randn(b, total, h * d)
+    cut = lambda t: t if fmt == "bshd" else t.transpose(0, 1)  # noqa: E731
+    with torch.no_grad():
+        full = cut(mha(cut(x), rotary_pos_emb=rope))
+        params = te.InferenceParams(4, 64, num_heads_kv=hk, head_dim_k=d, dtype=torch.float32, is_paged=True, page_size=16,
+                                    total_num_pages=16, qkv_format=fmt, device="cpu", cache_dtype=torch.float8_e4m3fn)
+        outs, pos = [], 0
+        for n in (7, 3, 1, 1, 8):
+            params.pre_step(OrderedDict((i, n) for i in range(b)))
+            outs.append(cut(mha(cut(x[:, pos:pos + n]), rotary_pos_emb=rope, inference_params=params)))
+            pos += n
+        # a ragged step: the second sequence is padded
+        params.truncate_sequence(0, 18)
+        params.truncate_sequence(1, 19)
+        params.pre_step(OrderedDict([(0, 2), (1, 1)]))
+        ragged = torch.stack([x[0, 18:20], torch.cat([x[1, 19:20], torch.full((1, h * d), 9.0)])])
+        again = cut(mha(cut(ragged), rotary_pos_emb=rope, inference_params=params))
+    inc = torch.cat(outs, dim=1)
+    assert (inc - full).norm() / full.norm() < 2.0 ** -3      # keys and values off by up to 2^-4 each
+    assert (again[0] - full[0, 18:20]).norm() / full[0, 18:20].norm() < 2.0 ** -3
+    assert (again[1, :1] - full[1, 19:20]).norm() / full[1, 19:20].norm() < 2.0 ** -3
+    with pytest.raises(RuntimeError, match="no backward"):
+        mha(cut(x[:, :1].repeat(1, 2, 1)), rotary_pos_emb=rope, inference_params=params)
+    params.pre_step(OrderedDict([(0, 1), (1, 1)]))
+    k, v = params.convert_paged_to_nonpaged(None)
+    assert k.shape == (2, 32, hk, d) and torch.isfinite(k).all()
+
+
+def test_variants_without_a_cache_kernel_read_expanded_keys():
+    torch.manual_seed(1)
+    attn = te.DotProductAttention(4, 16, num_gqa_groups=2, qkv_format="bshd", attn_mask_type="causal", softmax_type="off-by-one",
+                                  layer_number=1).eval()
+    params = te.InferenceParams(1, 64, num_heads_kv=2, head_dim_k=16, dtype=torch.float32, is_paged=True, page_size=16, total_num_pages=4,
+                                device="cpu", cache_dtype=torch.float8_e4m3fn)
+    q, k, v = torch.randn(1, 9, 4, 16), torch.exp2(torch.randint(-3, 3, (1, 9, 2, 16)).float()), torch.ones(1, 9, 2, 16)
+    with torch.no_grad():
+        params.pre_step(OrderedDict([(0, 9)]))
+        o = attn(q, k, v, inference_params=params)
+        torch.testing.assert_close(o, attn(q, k, v), rtol=1e-5, atol=1e-6)     # these keys and values are exact in 8 bits
+
+
+def test_generation_with_forks_and_an_8_bit_cache():
+    """The whole run: a windowed model with sinks decodes, forks a sequence, drops drafts, and the pool is compacted."""
+    from transformerengine_b200.models.mistral import MistralConfig, MistralModel
+    torch.manual_seed(2)
+    cfg = MistralConfig.tiny(params_dtype=torch.float32, sliding_window=24, sink_tokens=4)
+    model = MistralModel(cfg, device="cpu").eval()
+    prompt = torch.randint(0, cfg.vocab_size, (2, 40))
+    kw = dict(is_paged=True, page_size=16, total_num_pages=16)
+    out = model.generate(prompt, 20, cache_dtype=torch.float8_e4m3fn, **kw)
+    assert out.shape == (2, 60)
+    # logits against the full pass on the generated tokens: what the cache rounds moves them by a few percent
+    with torch.no_grad():
+        full = model(out).transpose(0, 1)
+        params = model.make_inference_params(4, 96, cache_dtype=torch.float8_e4m3fn, **kw)
+        assert params.cache_manager.window_size == 23 and params.cache_manager.sink_tokens == 4
+        params.pre_step(OrderedDict([(0, 50), (1, 50)]))
+        model(out[:, :50], inference_params=params)
+        params.fork_sequence(1, 7)
+        params.pre_step(OrderedDict([(0, 3), (1, 3), (7, 3)]))
+        model(torch.cat([out[:, 50:53], out[:1, 30:33]]), inference_params=params)
+        params.truncate_sequence(7, 50)
+        params.compact()
+        params.pre_step(OrderedDict([(1, 3), (7, 6)]))
+        step = torch.cat([torch.cat([out[1:, 53:56], out[1:, :3]], 1), out[1:, 50:56]])
+        logits = model(step, inference_params=params).transpose(0, 1)
+    for got, at in ((logits[0, :3], slice(53, 56)), (logits[1], slice(50, 56))):
+        assert (got - full[1, at]).norm() / full[1, at].norm() < 2.0 ** -3

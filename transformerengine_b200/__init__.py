@@ -22,7 +22,8 @@ from .modules.layernorm_mlp import LayerNormMLP
 from .attention.dot_product_attention import DotProductAttention
 from .attention.multi_head_attention import MultiheadAttention
 from .attention.rope import RotaryPositionEmbedding, apply_rotary_pos_emb
-from .attention.inference import InferenceParams, KVCacheManager, NonPagedKVCacheManager, PagedKVCacheManager
+from .attention.inference import (InferenceParams, KVCacheManager, NonPagedKVCacheManager, PagedKVCacheManager,
+                                  FP8PagedKVCacheManager)
 from .attention.fused_mla_q_uproj import FusedMLAQUpProjRopeQuant
 from .attention import thd  # noqa: F401  packed-sequence helpers
 from .attention import kv_cache  # noqa: F401  8-bit paged key/value cache

@@ -138,6 +138,11 @@ class DotProductAttention(torch.nn.Module):
             raise ValueError("score_mod_bprop without score_mod")
         if fp8 is not None:
             query_layer, key_layer, value_layer = fp8.inputs(query_layer, key_layer, value_layer)
+        if inference_params is not None and self._cache_attends(inference_params, query_layer, score_mod, window, mask_type,
+                                                                core_attention_bias_type):
+            out = inference_params.attend(self.layer_number, query_layer, key_layer, value_layer, fmt, mask_type,
+                                          scale=self.softmax_scale, window=window, sink_tokens=self.sink_tokens)
+            return out if fp8 is None else fp8.output(out)
         if inference_params is not None:
             query_layer, key_layer, value_layer, fmt, mask_type, cu_seqlens_q, cu_seqlens_kv = \
                 inference_params.step(self.layer_number, query_layer, key_layer, value_layer, fmt, mask_type)
@@ -163,6 +168,16 @@ class DotProductAttention(torch.nn.Module):
             out = inference_params.unpack_output(out)
         out = out if fp8 is None else fp8.output(out)
         return (out, self._max_logit) if self.return_max_logit else out
+
+    def _cache_attends(self, inference_params, q, score_mod, window, mask_type, bias_type) -> bool:
+        """Whether the cache's own attention covers this call; else it hands out expanded keys and values."""
+        causal = "causal" in mask_type
+        open_right = window is None or window[1] < 0 or (causal and window[1] == 0)
+        return getattr(inference_params, "attends", bool)() and self.softmax_type == "vanilla" and score_mod is None and \
+            bias_type == "no_bias" and not self.return_max_logit and open_right and \
+            (causal or window is None or window[0] < 0) and not (self.training and self.attention_dropout > 0.0) and \
+            (self.cp_group is None or D.get_world_size(self.cp_group) == 1) and \
+            (not q.is_cuda or q.dtype in (torch.bfloat16, torch.float16)) and q.shape[-1] <= 256
 
     _logged: set = set()
 

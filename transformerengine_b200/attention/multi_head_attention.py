@@ -39,7 +39,8 @@ class MultiheadAttention(torch.nn.Module):
                  qkv_format: str = "sbhd", name: Optional[str] = None, qk_norm_type: Optional[str] = None,
                  qk_norm_eps: float = 1e-6, qk_norm_before_rope: bool = False, seq_length: Optional[int] = None,
                  micro_batch_size: Optional[int] = None, softmax_type: str = "vanilla",
-                 rotary_pos_interleaved: bool = False, bottom_right_diagonal: Optional[bool] = None) -> None:
+                 rotary_pos_interleaved: bool = False, bottom_right_diagonal: Optional[bool] = None,
+                 sink_tokens: int = 0) -> None:
         super().__init__()
         self.rotary_pos_interleaved = rotary_pos_interleaved
         self.bottom_right_diagonal = bottom_right_diagonal
@@ -119,7 +120,7 @@ class MultiheadAttention(torch.nn.Module):
             attention_dropout=attention_dropout, qkv_format=qkv_format, tp_size=self.tp_size,
             get_rng_state_tracker=get_rng_state_tracker, sequence_parallel=sequence_parallel, tp_group=tp_group,
             layer_number=layer_number, attention_type=attention_type, attn_mask_type=attn_mask_type,
-            window_size=window_size, softmax_type=softmax_type)
+            window_size=window_size, softmax_type=softmax_type, sink_tokens=sink_tokens)
         self.proj = Linear(self.hidden_size_q, hidden_size, init_method=output_layer_init_method, bias=bias,
                            return_bias=return_bias, parallel_mode="row" if set_parallel_mode else None,
                            name=f"{name}.proj" if name else None, **common)

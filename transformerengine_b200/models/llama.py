@@ -42,6 +42,7 @@ class LlamaConfig:
     embedding_scale: Optional[float] = None   # multiply the token embeddings (Gemma: sqrt(hidden_size))
     tie_embeddings: bool = False              # the output head shares the embedding table
     sliding_window: Optional[int] = None      # attend to the last N tokens only (Mistral)
+    sink_tokens: int = 0                      # ... and to the first N tokens (streaming attention)
     qk_norm: bool = False                     # RMSNorm over each head of q and k, before the rotation (Qwen3)
     qk_norm_eps: float = 1e-6
 
@@ -194,6 +195,7 @@ class LlamaModel(torch.nn.Module):
                              layernorm_epsilon=cfg.rms_eps, hidden_dropout=0.0, attention_dropout=0.0,
                              init_method=init, output_layer_init_method=init, layer_number=i + 1,
                              kv_channels=cfg.head_dim, self_attn_mask_type="causal", window_size=window,
+                             sink_tokens=cfg.sink_tokens,
                              tp_group=tp_group, tp_size=self.tp_size,
                              params_dtype=cfg.params_dtype, sequence_parallel=self.sp,
                              set_parallel_mode=self.tp_size > 1, fuse_qkv_params=True, qkv_weight_interleaved=False,
@@ -225,11 +227,15 @@ class LlamaModel(torch.nn.Module):
 
     def make_inference_params(self, max_batch_size: int, max_sequence_length: int, **kw):
         """Key/value cache for incremental decoding with this model (``is_paged``, ``page_size``,
-        ``total_num_pages`` pass through to ``InferenceParams``)."""
+        ``total_num_pages``, ``cache_dtype`` pass through to ``InferenceParams``; an 8-bit cache is told the model's
+        sliding window and gives pages out of sight back)."""
         from ..attention.inference import InferenceParams
         cfg = self.cfg
         p = next(self.parameters())
         kw.setdefault("device", p.device)
+        if kw.get("cache_dtype") == torch.float8_e4m3fn and cfg.sliding_window:
+            kw.setdefault("window_size", cfg.sliding_window - 1)
+            kw.setdefault("sink_tokens", cfg.sink_tokens)
         return InferenceParams(max_batch_size, max_sequence_length, num_heads_kv=cfg.num_kv_heads // self.tp_size,
                                head_dim_k=cfg.dim_per_head, dtype=cfg.params_dtype,
                                qkv_format="sbhd", **kw)

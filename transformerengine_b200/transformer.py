@@ -58,7 +58,8 @@ class TransformerLayer(torch.nn.Module):
                  device: Union[torch.device, str] = None, attn_input_format: str = "sbhd", name: Optional[str] = None,
                  qk_norm_type: Optional[str] = None, qk_norm_eps: float = 1e-6, qk_norm_before_rope: bool = False,
                  softmax_type: str = "vanilla", bottom_right_diagonal: Optional[bool] = None,
-                 enc_dec_bottom_right_diagonal: Optional[bool] = None) -> None:
+                 enc_dec_bottom_right_diagonal: Optional[bool] = None, sink_tokens: int = 0) -> None:
+        """``sink_tokens``: first tokens that the self-attention still sees left of its sliding window."""
         super().__init__()
         self.bottom_right_diagonal = bottom_right_diagonal
         self.enc_dec_bottom_right_diagonal = enc_dec_bottom_right_diagonal
@@ -97,6 +98,7 @@ class TransformerLayer(torch.nn.Module):
         self.self_attention = MultiheadAttention(hidden_size, num_attention_heads, **attn_kwargs,
                                                  input_layernorm=not output_layernorm, attention_type="self",
                                                  attn_mask_type=self_attn_mask_type, window_size=window_size,
+                                                 sink_tokens=sink_tokens,
                                                  return_bias=not parallel_attention_mlp,
                                                  name=f"{name}.self_attention" if name else None)
         if layer_type == "decoder":
