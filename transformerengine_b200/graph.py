@@ -20,6 +20,8 @@ Without CUDA the callables are returned unchanged (eager).
 """
 from __future__ import annotations
 
+import contextlib
+import gc
 import warnings
 from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 
@@ -29,6 +31,21 @@ from .quantization import DelayedScalingRecipeState, FP8GlobalStateManager, auto
 
 
 _IS_GRAPH_CAPTURING = [False]
+
+
+@contextlib.contextmanager
+def _capture(graph, **kw):
+    """``torch.cuda.graph`` with the garbage collector held off: a dead graph that it destroys while another one is being
+    captured invalidates that capture."""
+    gc.collect()
+    was = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, **kw):
+            yield
+    finally:
+        if was:
+            gc.enable()
 
 
 def set_capture_start() -> None:
@@ -111,7 +128,7 @@ class GraphedStep:
         from .ops import _ext
 
         before = _ext.get().launch_count() if _ext.available() else 0
-        with torch.cuda.graph(self.graph, pool=pool, capture_error_mode="thread_local"):
+        with _capture(self.graph, pool=pool, capture_error_mode="thread_local"):
             out = self._run()
         self.kernels_per_replay = (_ext.get().launch_count() - before) if _ext.available() else 0
         self._is_tuple = isinstance(out, (tuple, list))
@@ -206,7 +223,7 @@ class _Graphed:
         old = freeze_weight_caches(self.cache_quantized_params)  # cached weights: no quantize kernels recorded
         try:
             self.fwd_graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.fwd_graph, pool=self.pool):
+            with _capture(self.fwd_graph, pool=self.pool):
                 out = self._call()
         finally:
             freeze_weight_caches(old)
@@ -218,7 +235,7 @@ class _Graphed:
         self.grad_targets = self._grad_inputs()
         need = [(o, g) for o, g in zip(self.static_out, self.static_gout) if g is not None]
         self.bwd_graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.bwd_graph, pool=self.pool):
+        with _capture(self.bwd_graph, pool=self.pool):
             self.static_gin = torch.autograd.grad([o for o, _ in need], self.grad_targets, [g for _, g in need],
                                                   allow_unused=True)
         if not self.allow_unused:
