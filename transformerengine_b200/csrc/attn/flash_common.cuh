@@ -56,6 +56,9 @@ struct FlashParams {
   // includes the right extent win_right) and, when has_lo, j >= i + lo_off
   int win_left, win_right, has_lo, lo_off;
   int n_sink;        // keys j < n_sink are visible left of the window too
+  int sink_chunks, sink_len;        // dK/dV pass: parts of the queries of a key block that holds sinks (see FlashArgs)
+  float* part_sink;
+  float* part_rest;
   int pair_balance;  // query-stationary kernels: a CTA takes 128-row tiles i and last - i (equal causal work)
 };
 

@@ -7,6 +7,9 @@
 //   dV += P^T dO,  dK += dS^T Q          (A operands from TMEM; dO and Q blocks reused as MN-major B)
 // Two groups of softmax warps alternate over the query blocks so that the tensor pipe and the
 // exponentials overlap.  dK/dV stay in TMEM for the whole walk and are written once.
+// With sinks left of a window the first key blocks are seen by all queries, the others by a window's worth: one CTA per
+// block would leave the sinks' CTA running alone (16 heads, 16384 tokens, window 512: 7x the others' work).  Their queries
+// are split over CTAs of about the others' length, and the partial sums (fp32) are joined by flash_bwd_join.
 #include "flash_common.cuh"
 #include "flash_qouter_softmax.cuh"
 
@@ -48,7 +51,15 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   // heads vary fastest, so CTAs start in order of decreasing causal work over ALL heads
-  const int kb = blockIdx.y;
+  int kb = blockIdx.y;
+  int chunk = 0;                          // which part of the queries, for key blocks with sinks
+  bool sink_block = false;
+  if (WIN == kWindowSinks) {
+    const int sb = (p_launch.n_sink + 127) / 128;
+    sink_block = kb < sb * p_launch.sink_chunks;
+    chunk = sink_block ? kb % p_launch.sink_chunks : 0;
+    kb = sink_block ? kb / p_launch.sink_chunks : kb - sb * p_launch.sink_chunks + sb;
+  }
   const int hk = static_cast<int>(blockIdx.x) / p_launch.gsplit;
   const int gs = static_cast<int>(blockIdx.x) % p_launch.gsplit;  // which part of the head group
   const int b = blockIdx.z;
@@ -69,6 +80,10 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   if (p.causal) {
     const int first_q = kv0 - p.causal_off;  // first query row that sees key kv0
     i_start = first_q <= 0 ? 0 : first_q / 64;
+  }
+  if (WIN == kWindowSinks && sink_block && p.sink_chunks > 1) {
+    i_start = max(i_start, chunk * p.sink_len);
+    nq = min(nq, (chunk + 1) * p.sink_len);
   }
   const int ni = nq > i_start ? nq - i_start : 0;
   const int N = Gl * ni;
@@ -266,6 +281,15 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                        static_cast<long long>(kv_row) * p.o_ss + half * 64;
       const float mul = u == 0 ? p.scale : 1.f;
       const uint32_t col0 = (u == 0 ? C::kColDk : C::kColDv) + half * 64;
+      float* part = nullptr;
+      if (WIN == kWindowSinks && (sink_block ? p.part_sink : p.part_rest) != nullptr) {
+        const int edge = (p_launch.n_sink + 127) / 128 * 128;   // rows in sink blocks
+        const int which = sink_block ? gs * p.sink_chunks + chunk : gs;
+        const long long rows = sink_block ? edge : p_launch.sk - edge;
+        part = (sink_block ? p.part_sink : p.part_rest) +
+               (((static_cast<long long>(which) * p.b + b) * p.hk + hk) * rows + (sink_block ? kv_row : kv_row - edge)) * 256 +
+               (u == 0 ? 0 : 128) + half * 64;
+      }
 #pragma unroll 1
       for (int c0 = 0; c0 < 64; c0 += 32) {
         uint32_t o[32];
@@ -276,7 +300,15 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #pragma unroll
           for (int c = 0; c < 32; ++c) o[c] = 0u;
         }
-        if (row_ok) {
+        if (WIN == kWindowSinks && part != nullptr) {
+          if (row_ok) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              *reinterpret_cast<float4*>(part + c0 + c) =
+                  make_float4(__uint_as_float(o[c]) * mul, __uint_as_float(o[c + 1]) * mul, __uint_as_float(o[c + 2]) * mul,
+                              __uint_as_float(o[c + 3]) * mul);
+          }
+        } else if (row_ok) {
 #pragma unroll
           for (int c = 0; c < 32; c += 8) {
             uint32_t q4[4];
@@ -296,6 +328,39 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
+}
+
+// Adds the fp32 parts of a key row's dK and dV and rounds them: one warp per row, lanes 0 - 15 dK, 16 - 31 dV.
+template <bool BF>
+__global__ void __launch_bounds__(256) flash_bwd_join_kernel(const FlashParams p_launch, int rows) {
+  FlashParams p = p_launch;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const SeqView sv = localize(p, b);
+  const int edge = (p_launch.n_sink + 127) / 128 * 128;
+  if (row >= rows || row >= p.sk) return;
+  const bool sink = row < edge;
+  const float* part = sink ? p.part_sink : p.part_rest;
+  if (part == nullptr) return;
+  const int parts = sink ? p.gsplit * p.sink_chunks : p.gsplit;
+  const long long span = sink ? edge : p_launch.sk - edge;
+  const long long step = static_cast<long long>(p.b) * p.hk * span * 256;
+  part += ((static_cast<long long>(b) * p.hk + hk) * span + (sink ? row : row - edge)) * 256 + lane * 8;
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(part + s * step);
+    const float4 y = *reinterpret_cast<const float4*>(part + s * step + 4);
+    acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
+    acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
+  }
+  uint16_t* out = reinterpret_cast<uint16_t*>(lane < 16 ? p.out : p.out2) + b * p.o_sb + hk * p.o_sh +
+                  static_cast<long long>(sv.k_off + row) * p.o_ss + (lane & 15) * 8;
+  *reinterpret_cast<uint4*>(out) = make_uint4(pack16<BF>(acc[0], acc[1]), pack16<BF>(acc[2], acc[3]),
+                                              pack16<BF>(acc[4], acc[5]), pack16<BF>(acc[6], acc[7]));
 }
 
 // delta[b, h, s] = sum_d dO * O, one warp per row
@@ -371,7 +436,11 @@ cudaError_t flash_bwd_dkdv(const FlashArgs& a, cudaStream_t stream) {
   p.lse = a.lse; p.delta = a.delta; p.s_pad = a.s_pad; p.status = a.status;
   p.cu_q = a.cu_q; p.cu_k = a.cu_k; p.off_q = a.off_q; p.off_k = a.off_k;
   p.gsplit = a.gsplit < 1 ? 1 : a.gsplit;
-  p.o_sg = a.dk_sg;
+  p.o_sg = a.part_rest != nullptr ? 0 : a.dk_sg;
+  p.sink_chunks = a.sink_chunks; p.sink_len = a.sink_len; p.part_sink = a.part_sink; p.part_rest = a.part_rest;
+  if (p.n_sink > 0 && p.has_lo && (a.sink_chunks < 1 || (a.sink_chunks * p.gsplit > 1 && a.part_sink == nullptr) ||
+                                   (p.gsplit > 1 && a.part_rest == nullptr && (p.n_sink + 127) / 128 * 128 < a.sk)))
+    return cudaErrorInvalidValue;
   if ((a.hq / a.hk) % p.gsplit != 0 || p.o_sg % 8 != 0) return cudaErrorInvalidValue;
   static bool attr_set = false;
   if (!attr_set) {
@@ -387,12 +456,57 @@ cudaError_t flash_bwd_dkdv(const FlashArgs& a, cudaStream_t stream) {
     }
     attr_set = true;
   }
-  dim3 grid(a.hk * p.gsplit, (a.sk + 127) / 128, a.b);
+  const int sink_blocks = mask_variant(p) == kWindowSinks ? (p.n_sink + 127) / 128 : 0;
+  dim3 grid(a.hk * p.gsplit, (a.sk + 127) / 128 + sink_blocks * (a.sink_chunks - 1), a.b);
   const auto go = [&](auto kernel) { kernel<<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, tdo, p); };
   const int win = mask_variant(p);
   if (win == kNoWindow) bf ? go(flash_kvouter_kernel<true, kNoWindow>) : go(flash_kvouter_kernel<false, kNoWindow>);
   else if (win == kWindow) bf ? go(flash_kvouter_kernel<true, kWindow>) : go(flash_kvouter_kernel<false, kWindow>);
   else bf ? go(flash_kvouter_kernel<true, kWindowSinks>) : go(flash_kvouter_kernel<false, kWindowSinks>);
+  return cudaGetLastError();
+}
+
+long long flash_sink_plan(FlashArgs& a, bool allow_gsplit, long long* sink_floats) {
+  *sink_floats = 0;
+  a.gsplit = a.sink_chunks = 1;
+  if (a.sq <= 0 || a.sk <= 0 || a.b <= 0) return 0;
+  const int n_sink = a.sink_tokens < a.sk ? a.sink_tokens : a.sk;
+  const long long sink_blocks = (n_sink + 127) / 128, blocks = (a.sk + 127) / 128;
+  const long long heads = static_cast<long long>(a.hk) * a.b;
+  // about as many 64-row query blocks as a key block of the window has; no more parts than fill the SMs twice
+  const long long right = a.causal ? 0 : (a.window_right >= 0 ? a.window_right : a.sq);
+  long long len = (static_cast<long long>(a.window_left) + right + 128) / 64 + 2;
+  const long long all = (a.sq + 63) / 64;
+  const long long most = (2 * 148 + sink_blocks * heads - 1) / (sink_blocks * heads);
+  long long chunks = (all + len - 1) / len;
+  chunks = chunks < most ? chunks : most;
+  chunks = chunks < 1 ? 1 : chunks;
+  a.sink_len = static_cast<int>((all + chunks - 1) / chunks);
+  a.sink_chunks = static_cast<int>((all + a.sink_len - 1) / a.sink_len);
+  const int group = a.hq / a.hk;
+  a.gsplit = allow_gsplit && group > 1 && (blocks + sink_blocks * (a.sink_chunks - 1)) * heads < 2 * 148 ? group : 1;
+  a.dk_sg = 0;
+  const long long parts = static_cast<long long>(a.gsplit) * a.sink_chunks;
+  *sink_floats = parts > 1 ? parts * heads * sink_blocks * 128 * 256 : 0;
+  const long long rest = a.gsplit > 1 && blocks > sink_blocks ? a.gsplit * heads * (a.sk - sink_blocks * 128) * 256 : 0;
+  return *sink_floats + rest;
+}
+
+cudaError_t flash_bwd_join(const FlashArgs& a, cudaStream_t stream) {
+  using namespace attn;
+  if (a.part_sink == nullptr || a.b <= 0 || a.sk <= 0) return cudaSuccess;
+  FlashParams p = {};
+  p.b = a.b; p.hq = a.hq; p.hk = a.hk; p.sq = a.sq; p.sk = a.sk;
+  set_mask_params(p, a);
+  p.out = a.dk; p.out2 = a.dv; p.o_sb = a.dk_sb; p.o_sh = a.dk_sh; p.o_ss = a.dk_ss;
+  p.cu_q = a.cu_q; p.cu_k = a.cu_k; p.off_q = a.off_q; p.off_k = a.off_k;
+  p.gsplit = a.gsplit; p.sink_chunks = a.sink_chunks; p.sink_len = a.sink_len;
+  p.part_sink = a.part_sink; p.part_rest = a.part_rest;
+  const int edge = (p.n_sink + 127) / 128 * 128;
+  const int rows = a.part_rest != nullptr ? a.sk : (edge < a.sk ? edge : a.sk);
+  const dim3 grid((rows + 7) / 8, a.hk, a.b);
+  if (a.is_bf16) flash_bwd_join_kernel<true><<<grid, 256, 0, stream>>>(p, rows);
+  else flash_bwd_join_kernel<false><<<grid, 256, 0, stream>>>(p, rows);
   return cudaGetLastError();
 }
 

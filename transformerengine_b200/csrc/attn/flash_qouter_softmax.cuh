@@ -76,10 +76,30 @@ __device__ __forceinline__ void qouter_softmax_role(const FlashParams& p, uint8_
     const int kv0 = kb0 + half * HC;      // first key of this thread's columns
     const bool need_mask = (kb0 + BK > p.sk) || (p.causal && kb0 + BK - 1 > q0 + t * 128 + p.causal_off) ||
                            (WIN && kb0 < q0 + t * 128 + 127 + p.lo_off);
-    const int lim = p.causal ? min(p.sk - 1, q_row + p.causal_off) : p.sk - 1;  // last visible key
-    const int lo = WIN ? q_row + p.lo_off : 0;                                 // first visible key
-    const int sinks = WIN == kWindowSinks ? p.n_sink : 0;                      // but these see left of it
-    const auto hidden = [&](int key) { return key > lim || (key < lo && (WIN != kWindowSinks || key >= sinks)); };
+    int lim = p.causal ? min(p.sk - 1, q_row + p.causal_off) : p.sk - 1;       // last visible key
+    int lo = WIN ? q_row + p.lo_off : 0;                                       // first visible key
+    if (WIN == kWindowSinks && kb0 < p.n_sink) {
+      // A block that holds sinks.  A row whose window has not left them sees keys 0 .. lim, one whose window lies behind
+      // the block the sinks alone: one range either way, as in any other block.  Where sinks and window both lie in the
+      // block with a gap between them, the gap's scores are overwritten first.
+      const bool gap = lo > p.n_sink && lo < kb0 + BK;
+      if (lo >= kb0 + BK) lim = min(lim, p.n_sink - 1);
+      if (__any_sync(0xffffffffu, gap)) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < HC; c0 += 32) {
+          uint32_t s[32];
+          tmem_ld_32x32(col_s + c0, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (gap && kv0 + c0 + c >= p.n_sink && kv0 + c0 + c < lo) s[c] = __float_as_uint(NEG_INF);
+          tmem_st_32x32(col_s + c0, s);
+        }
+        tmem_st_wait();
+      }
+      lo = 0;
+    }
+    const auto hidden = [&](int key) { return key > lim || key < lo; };
     if (MODE == kModeFwd) {
       // pass 1: block maximum of this thread's columns, 32 at a time
       float mx4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};

@@ -179,6 +179,22 @@ void run_dkdv(teb200::FlashArgs& a, const at::Tensor& k, const at::Tensor& dk, c
     const char* e = std::getenv("TEB200_ATTN_GSPLIT");
     return e == nullptr || e[0] != '0';
   }();
+  if (a.window_left >= 0 && a.sink_tokens > 0) {
+    // sinks: parts in fp32, added and rounded by a kernel of their own
+    long long sink_floats = 0;
+    const long long need = teb200::flash_sink_plan(a, allow_split, &sink_floats);
+    at::Tensor parts;
+    if (need > 0) {
+      parts = at::empty({static_cast<int64_t>(need)}, dk.options().dtype(at::kFloat));
+      a.part_sink = parts.data_ptr<float>();
+      a.part_rest = need > sink_floats ? a.part_sink + sink_floats : nullptr;
+    }
+    cudaError_t e = teb200::flash_bwd_dkdv(a, cur_stream());
+    TORCH_CHECK(e == cudaSuccess, "flash_bwd_dkdv (sinks) failed: ", cudaGetErrorString(e));
+    e = teb200::flash_bwd_join(a, cur_stream());
+    TORCH_CHECK(e == cudaSuccess, "flash_bwd_join failed: ", cudaGetErrorString(e));
+    return;
+  }
   if (allow_split && group > 1 && ctas < 2 * 148) {
     auto opts = dk.options();
     std::vector<int64_t> shape = {group, k.size(0), k.size(1), k.size(2), 128};

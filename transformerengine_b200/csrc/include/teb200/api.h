@@ -101,7 +101,16 @@ struct FlashArgs {
   int window_left = -1, window_right = -1;
   // Left of the window the first sink_tokens keys stay visible (0: none; only read with window_left >= 0).
   int sink_tokens = 0;
+  // dK/dV pass with sinks: every query sees the key blocks that hold them, so their queries are split over sink_chunks
+  // CTAs of sink_len 64-row blocks.  These CTAs, and all of them with gsplit > 1, leave fp32 partial sums
+  // [part][b][hk][rows][dK 128, dV 128] that flash_bwd_join adds and rounds once.
+  int sink_chunks = 1, sink_len = 0;
+  float* part_sink = nullptr;  // gsplit * sink_chunks parts of the rows in sink blocks (nullptr: one part, written directly)
+  float* part_rest = nullptr;  // gsplit parts of the other rows (nullptr: gsplit == 1)
 };
+// Fills gsplit / sink_chunks / sink_len for the dK/dV pass with sinks; returns the workspace in floats (part_sink first).
+long long flash_sink_plan(FlashArgs& args, bool allow_gsplit, long long* sink_floats);
+cudaError_t flash_bwd_join(const FlashArgs& args, cudaStream_t stream);
 cudaError_t flash_fwd(const FlashArgs& args, cudaStream_t stream);
 cudaError_t flash_delta(const FlashArgs& args, cudaStream_t stream);     // delta = rowsum(dO * O)
 cudaError_t flash_bwd_dq(const FlashArgs& args, cudaStream_t stream);
