@@ -59,10 +59,6 @@ def _cuda(cache: FP8KVCache) -> bool:
     return cache.k.is_cuda
 
 
-def _status(t: torch.Tensor) -> torch.Tensor:
-    return _ext.get().status(t.device.index)
-
-
 # ------------------------------------------------------------------------------------------------ reference pieces
 def block_scale(top: torch.Tensor) -> torch.Tensor:
     """The smallest power of two with ``top <= 448 * scale``, within 2^-60 .. 2^60 (2^-60 for zero)."""
@@ -147,7 +143,7 @@ def append(cache: FP8KVCache, new_k: torch.Tensor, new_v: torch.Tensor, page_tab
         _append_ref(cache, new_k, new_v, page_table, cu_new, kv_lens)
         return
     _ext.get().fp8_cache_append(*cache, new_k, new_v, page_table, cu_new, kv_lens,
-                                new_k.shape[0] if max_new is None else max_new, _status(cache.k))
+                                new_k.shape[0] if max_new is None else max_new)
 
 
 def gather(cache: FP8KVCache, page_table: torch.Tensor, kv_lens: torch.Tensor, offsets: torch.Tensor, rows: int,
@@ -158,8 +154,7 @@ def gather(cache: FP8KVCache, page_table: torch.Tensor, kv_lens: torch.Tensor, o
     k = torch.empty(rows, h, d, dtype=dtype, device=cache.k.device)
     v = torch.empty_like(k)
     if _cuda(cache):
-        _ext.get().fp8_cache_gather(*cache, page_table, kv_lens, offsets, k, v, 0, rows if max_kv is None else max_kv,
-                                    _status(cache.k))
+        _ext.get().fp8_cache_gather(*cache, page_table, kv_lens, offsets, k, v, 0, rows if max_kv is None else max_kv)
         return k, v
     for i, (n, o, pages) in enumerate(zip(kv_lens.tolist(), offsets.tolist(), page_table.tolist())):
         k[o:o + n], v[o:o + n] = _values_ref(cache, pages, n, dtype)
@@ -196,8 +191,7 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
     hq, hk, d = q.shape[1], cache.k.shape[1], q.shape[2]
     if d == 128 and hq // hk * max_q > _DIRECT_ROWS and max_kv > 0 and q.dtype in (torch.bfloat16, torch.float16):
         return _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
-    return _ext.get().fp8_cache_attend(q, *cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens,
-                                       _status(q))
+    return _ext.get().fp8_cache_attend(q, *cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
 
 
 def _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens):
@@ -209,7 +203,7 @@ def _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, 
     off = torch.arange(0, (n + 1) * pitch, pitch, dtype=torch.int32, device=q.device)
     k = torch.empty(n * pitch, h, d, dtype=q.dtype, device=q.device)
     v = torch.empty_like(k)
-    C_.fp8_cache_gather(*cache, page_table, kv_lens, off, k, v, pitch, max_kv, _status(q))
+    C_.fp8_cache_gather(*cache, page_table, kv_lens, off, k, v, pitch, max_kv)
     cu_k = torch.zeros(n + 1, dtype=torch.int32, device=q.device)
     torch.cumsum(kv_lens, 0, dtype=torch.int32, out=cu_k[1:])
     return _flash.flash_varlen_forward(q, k, v, cu_q, cu_k, cu_q, off, max_q, max_kv, scale, causal, left, sink_tokens)

@@ -1,7 +1,8 @@
 // 8-bit paged key/value cache: quantizing append, dequantizing gather, page copies.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
+
+#include <type_traits>
 
 #include "fp8_cache.cuh"
 #include "teb200/api.h"
@@ -12,52 +13,54 @@ namespace {
 
 using namespace kvc;
 
-// 8 consecutive values of a row as fp32
+// 8 consecutive values of a row, as they are loaded and as fp32
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+struct Raw8 {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p + i);
-    x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
   }
-}
+};
 template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 v = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 4);
   }
-}
-template <>
-__device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
-  const uint4 v = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   }
-}
+};
 
-// One warp per (sequence, 16-token block, head, K or V).  A lane owns 8 consecutive dims of the rows lane / (d / 8),
-// + 32 / (d / 8), ...; the block's largest finite magnitude sets the scale, and rows that were there before are rounded
-// again when it rises.  A power-of-two scale makes that second rounding exact except where a code becomes subnormal.
+// One warp per (sequence, 16-token block, K or V, head); the four warps of a CTA take neighbouring heads, whose rows
+// adjoin in memory.  A lane owns 8 consecutive dims of the rows lane / (d / 8), + 32 / (d / 8), ...  The block's largest
+// finite magnitude sets the scale, and rows that were there before are rounded again when it rises.  A power-of-two scale
+// makes that second rounding exact except where a code becomes subnormal.  Reading 16-bit rows and writing codes bounds
+// long runs; a single token per sequence is one chain of dependent loads (lengths, then page and row, then scale).
 template <typename T, int D>
 __global__ void __launch_bounds__(128) append_kernel(const Fp8AppendArgs a) {
   constexpr int kLanesPerRow = D / 8;
   constexpr int kRows = 32 / kLanesPerRow;   // rows per pass
   constexpr int kPasses = kKvBlock / kRows;
   const int lane = threadIdx.x & 31;
-  const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);  // (head, K or V)
+  const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (unit >= 2 * a.c.heads) return;
-  const int head = unit >> 1;
-  const bool is_v = unit & 1;
+  const bool is_v = unit >= a.c.heads;
+  const int head = is_v ? unit - a.c.heads : unit;
   const int seq = blockIdx.z;
   const int per = a.c.page_size / kKvBlock;
   const int src0 = a.cu_new[seq];
@@ -75,6 +78,15 @@ __global__ void __launch_bounds__(128) append_kernel(const Fp8AppendArgs a) {
   for (int blk = old / kKvBlock + blockIdx.y; blk * kKvBlock < len; blk += gridDim.y) {
     const int slot = blk / per;
     const int page = slot < a.c.width ? a.c.table[static_cast<long long>(seq) * a.c.width + slot] : -1;
+    const int first = max(old - blk * kKvBlock, 0);             // rows [first, end) are new
+    const int end = min(len - blk * kKvBlock, kKvBlock);
+    const T* rows = src + (src0 + blk * kKvBlock - old) * st;
+    Raw8<T> raw[kPasses];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int r = p * kRows + lane / kLanesPerRow;
+      if (r >= first && r < end) raw[p].load(rows + r * st);
+    }
     if (page < 0 || page >= a.c.pages) {
       if (lane == 0) atomicCAS(a.c.status, 0, kKvStatusPages);
       continue;
@@ -82,32 +94,25 @@ __global__ void __launch_bounds__(128) append_kernel(const Fp8AppendArgs a) {
     const long long idx = (static_cast<long long>(page) * a.c.heads + head) * per + blk % per;
     uint8_t* codes = (is_v ? a.c.v : a.c.k) + idx * (kKvBlock * D) + lane * 8;
     float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + idx;
-    const int first = max(old - blk * kKvBlock, 0);             // rows [first, end) are new
-    const int end = min(len - blk * kKvBlock, kKvBlock);
-    const T* rows = src + (src0 + blk * kKvBlock - old) * st;
-    float x[kPasses][8];
+    float was = first > 0 ? *scale : 0.f;
     float top = 0.f;
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int r = p * kRows + lane / kLanesPerRow;
       if (r >= first && r < end) {
-        load8<T>(rows + r * st, x[p]);
+        float x[8];
+        raw[p].get(x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float m = fabsf(x[p][i]);
+          const float m = fabsf(x[i]);
           if (m < INFINITY) top = fmaxf(top, m);                // NaN and infinities do not set the scale
         }
       }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float now = scale_for(top);
-    float was = now;
-    if (first > 0) {
-      was = *scale;
-      now = fmaxf(now, was);
-    }
-    __syncwarp();
+    const float now = fmaxf(scale_for(top), was);
+    if (first == 0) was = now;
     const float inv = inverse_of_power(now);
     const float again = was * inv;
 #pragma unroll
@@ -115,9 +120,11 @@ __global__ void __launch_bounds__(128) append_kernel(const Fp8AppendArgs a) {
       const int r = p * kRows + lane / kLanesPerRow;
       uint2* dst = reinterpret_cast<uint2*>(codes + p * 256);
       if (r >= first && r < end) {
+        float x[8];
+        raw[p].get(x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[p][i] *= inv;
-        *dst = make_uint2(to_e4m3x4(x[p][0], x[p][1], x[p][2], x[p][3]), to_e4m3x4(x[p][4], x[p][5], x[p][6], x[p][7]));
+        for (int i = 0; i < 8; ++i) x[i] *= inv;
+        *dst = make_uint2(to_e4m3x4(x[0], x[1], x[2], x[3]), to_e4m3x4(x[4], x[5], x[6], x[7]));
       } else if (r < first && now != was) {
         const uint2 old8 = *dst;
         float y[8];
@@ -128,7 +135,7 @@ __global__ void __launch_bounds__(128) append_kernel(const Fp8AppendArgs a) {
         *dst = make_uint2(to_e4m3x4(y[0], y[1], y[2], y[3]), to_e4m3x4(y[4], y[5], y[6], y[7]));
       }
     }
-    if (lane == 0) *scale = now;
+    if (lane == 0) *scale = now;   // every lane has read it: the maximum above is a warp-wide exchange
   }
 }
 
@@ -150,7 +157,7 @@ __device__ __forceinline__ void store8<__half>(__half* p, const float (&y)[8]) {
                                             pack2<false>(y[4], y[5]), pack2<false>(y[6], y[7]));
 }
 
-// One warp per (sequence, 16-token block, head, K or V): codes * scale into a token-major buffer.  Blocks whose page is
+// One warp per (sequence, 16-token block, K or V, head): codes * scale into a token-major buffer.  Blocks whose page is
 // not held, and the rows from a sequence's end to the next multiple of 128 (zero_to), become zeros.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
@@ -160,8 +167,8 @@ __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
   const int lane = threadIdx.x & 31;
   const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (unit >= 2 * a.c.heads) return;
-  const int head = unit >> 1;
-  const bool is_v = unit & 1;
+  const bool is_v = unit >= a.c.heads;
+  const int head = is_v ? unit - a.c.heads : unit;
   const int seq = blockIdx.z;
   const int per = a.c.page_size / kKvBlock;
   const int len = a.c.kv_lens[seq];

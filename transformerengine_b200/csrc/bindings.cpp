@@ -454,6 +454,9 @@ void rope(const at::Tensor& x, at::Tensor& out, const at::Tensor& freqs, int64_t
 
 }  // namespace
 
+// Status word of a device, for the other translation units.
+int* device_status(int device) { return status_tensor(device).data_ptr<int>(); }
+
 void register_extra(py::module_& m);  // bindings of kernels added in other translation units
 void register_kv(py::module_& m);     // bindings_kv.cpp
 

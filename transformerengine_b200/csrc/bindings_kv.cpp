@@ -12,6 +12,8 @@
 
 namespace py = pybind11;
 
+int* device_status(int device);   // bindings.cpp
+
 namespace {
 
 // numbers go into messages as strings (formatting one through a stream inside a check is not safe with every C++ runtime)
@@ -35,7 +37,7 @@ const int* int_vec(const at::Tensor& t, int64_t n, const at::Device& dev, const 
 }
 
 teb200::Fp8CacheView cache_view(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
-                                const at::Tensor& table, const at::Tensor& kv_lens, const at::Tensor& status) {
+                                const at::Tensor& table, const at::Tensor& kv_lens) {
   TORCH_CHECK(k.is_cuda() && k.dim() == 4 && k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes() &&
                   v.device() == k.device(),
               "the cache must be contiguous [pages, heads, page_size, d] codes, k and v alike");
@@ -68,7 +70,7 @@ teb200::Fp8CacheView cache_view(const at::Tensor& k, const at::Tensor& v, const 
   c.width = static_cast<int>(table.size(1));
   c.n = static_cast<int>(table.size(0));
   c.kv_lens = int_vec(kv_lens, table.size(0), k.device(), "kv_lens");
-  c.status = status.data_ptr<int>();
+  c.status = device_status(k.get_device());
   return c;
 }
 
@@ -84,10 +86,10 @@ at::Tensor rows16(const at::Tensor& t) {
 
 void fp8_cache_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
                       const at::Tensor& new_k, const at::Tensor& new_v, const at::Tensor& table, const at::Tensor& cu_new,
-                      const at::Tensor& kv_lens, int64_t max_new, const at::Tensor& status) {
+                      const at::Tensor& kv_lens, int64_t max_new) {
   c10::cuda::CUDAGuard guard(k.device());
   teb200::Fp8AppendArgs a;
-  a.c = cache_view(k, v, ks, vs, table, kv_lens, status);
+  a.c = cache_view(k, v, ks, vs, table, kv_lens);
   TORCH_CHECK(new_k.dim() == 3 && new_v.sizes() == new_k.sizes() && new_k.size(1) == a.c.heads && new_k.size(2) == a.c.d,
               "new keys and values must be [tokens, ", str(a.c.heads), ", ", str(a.c.d), "]");
   TORCH_CHECK(new_k.device() == k.device() && new_v.device() == k.device() && new_v.scalar_type() == new_k.scalar_type(),
@@ -108,10 +110,10 @@ void fp8_cache_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor
 
 void fp8_cache_gather(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
                       const at::Tensor& table, const at::Tensor& kv_lens, const at::Tensor& off, const at::Tensor& out_k,
-                      const at::Tensor& out_v, int64_t zero_to, int64_t max_kv, const at::Tensor& status) {
+                      const at::Tensor& out_v, int64_t zero_to, int64_t max_kv) {
   c10::cuda::CUDAGuard guard(k.device());
   teb200::Fp8GatherArgs a;
-  a.c = cache_view(k, v, ks, vs, table, kv_lens, status);
+  a.c = cache_view(k, v, ks, vs, table, kv_lens);
   TORCH_CHECK(out_k.dim() == 3 && out_k.sizes() == out_v.sizes() && out_k.is_contiguous() && out_v.is_contiguous() &&
                   out_k.size(1) == a.c.heads && out_k.size(2) == a.c.d && out_k.scalar_type() == out_v.scalar_type() &&
                   out_k.device() == k.device() && out_v.device() == k.device() && out_k.size(0) <= INT_MAX,
@@ -130,11 +132,10 @@ void fp8_cache_gather(const at::Tensor& k, const at::Tensor& v, const at::Tensor
 
 at::Tensor fp8_cache_attend(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
                             const at::Tensor& vs, const at::Tensor& table, const at::Tensor& cu_q, const at::Tensor& kv_lens,
-                            int64_t max_q, int64_t max_kv, double scale, bool causal, int64_t window_left, int64_t sinks,
-                            const at::Tensor& status) {
+                            int64_t max_q, int64_t max_kv, double scale, bool causal, int64_t window_left, int64_t sinks) {
   c10::cuda::CUDAGuard guard(k.device());
   teb200::Fp8AttendArgs a;
-  a.c = cache_view(k, v, ks, vs, table, kv_lens, status);
+  a.c = cache_view(k, v, ks, vs, table, kv_lens);
   TORCH_CHECK(q.dim() == 3 && q.size(2) == a.c.d && q.size(1) % a.c.heads == 0 && q.size(1) > 0,
               "queries must be [tokens, heads, ", str(a.c.d), "] with a multiple of the cache's ", str(a.c.heads), " heads");
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "queries must be fp16 or bf16");
