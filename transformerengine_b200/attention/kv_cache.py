@@ -154,7 +154,7 @@ def gather(cache: FP8KVCache, page_table: torch.Tensor, kv_lens: torch.Tensor, o
     k = torch.empty(rows, h, d, dtype=dtype, device=cache.k.device)
     v = torch.empty_like(k)
     if _cuda(cache):
-        _ext.get().fp8_cache_gather(*cache, page_table, kv_lens, offsets, k, v, 0, rows if max_kv is None else max_kv)
+        _ext.get().fp8_cache_gather(*cache, page_table, kv_lens, offsets, k, v, rows if max_kv is None else max_kv)
         return k, v
     for i, (n, o, pages) in enumerate(zip(kv_lens.tolist(), offsets.tolist(), page_table.tolist())):
         k[o:o + n], v[o:o + n] = _values_ref(cache, pages, n, dtype)
@@ -197,16 +197,8 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
 def _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens):
     """Codes expanded to 16 bits (every sequence padded to whole 128-token blocks with zeros), then the packed attention
     kernel: prompt chunks are bound by its products, not by the cache."""
-    C_ = _ext.get()
-    n, h, d = page_table.shape[0], cache.k.shape[1], cache.k.shape[3]
-    pitch = -(-max_kv // 128) * 128
-    off = torch.arange(0, (n + 1) * pitch, pitch, dtype=torch.int32, device=q.device)
-    k = torch.empty(n * pitch, h, d, dtype=q.dtype, device=q.device)
-    v = torch.empty_like(k)
-    C_.fp8_cache_gather(*cache, page_table, kv_lens, off, k, v, pitch, max_kv)
-    cu_k = torch.zeros(n + 1, dtype=torch.int32, device=q.device)
-    torch.cumsum(kv_lens, 0, dtype=torch.int32, out=cu_k[1:])
-    return _flash.flash_varlen_forward(q, k, v, cu_q, cu_k, cu_q, off, max_q, max_kv, scale, causal, left, sink_tokens)
+    k, v, out, cu_k, first = _ext.get().fp8_cache_expand(q, *cache, page_table, cu_q, kv_lens, max_kv, left, sink_tokens)
+    return _flash.flash_varlen_forward(q, k, v, out, cu_q, cu_k, cu_q, first, max_q, max_kv, scale, causal, left, sink_tokens)
 
 
 def copy_pages(caches: Sequence[Union[torch.Tensor, FP8KVCache]], src: Union[Sequence[int], torch.Tensor],

@@ -32,6 +32,21 @@ struct Raw8 {
       }
     }
   }
+  // larger of `top` and the magnitudes' bits, two 16-bit numbers at a time (their order is that of the values)
+  __device__ __forceinline__ uint32_t top_bits(uint32_t top) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+    return top;
+  }
+  static __device__ __forceinline__ bool finite(uint32_t top) {
+    constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+    return (top & 0xffffu) < kInf && (top >> 16) < kInf;
+  }
+  static __device__ __forceinline__ float value(uint32_t top) {
+    const uint16_t b = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+    return std::is_same<T, __nv_bfloat16>::value ? __uint_as_float(static_cast<uint32_t>(b) << 16) : __half2float(__ushort_as_half(b));
+  }
 };
 template <>
 struct Raw8<float> {
@@ -44,6 +59,15 @@ struct Raw8<float> {
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   }
+  __device__ __forceinline__ uint32_t top_bits(uint32_t top) const {
+    float x[8];
+    get(x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    return top;
+  }
+  static __device__ __forceinline__ bool finite(uint32_t top) { return top < 0x7f800000u; }
+  static __device__ __forceinline__ float value(uint32_t top) { return __uint_as_float(top); }
 };
 
 // One warp per (sequence, 16-token block, K or V, head); the four warps of a CTA take neighbouring heads, whose rows
@@ -52,7 +76,7 @@ struct Raw8<float> {
 // makes that second rounding exact except where a code becomes subnormal.  Reading 16-bit rows and writing codes bounds
 // long runs; a single token per sequence is one chain of dependent loads (lengths, then page and row, then scale).
 template <typename T, int D>
-__global__ void __launch_bounds__(128) append_kernel(const Fp8AppendArgs a) {
+__global__ void __launch_bounds__(128, D == 256 ? (sizeof(T) == 4 ? 2 : 4) : (sizeof(T) == 4 ? 4 : 8)) append_kernel(const Fp8AppendArgs a) {
   constexpr int kLanesPerRow = D / 8;
   constexpr int kRows = 32 / kLanesPerRow;   // rows per pass
   constexpr int kPasses = kKvBlock / kRows;
@@ -95,17 +119,25 @@ __global__ void __launch_bounds__(128) append_kernel(const Fp8AppendArgs a) {
     uint8_t* codes = (is_v ? a.c.v : a.c.k) + idx * (kKvBlock * D) + lane * 8;
     float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + idx;
     float was = first > 0 ? *scale : 0.f;
-    float top = 0.f;
+    uint32_t bits = 0;
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
       const int r = p * kRows + lane / kLanesPerRow;
-      if (r >= first && r < end) {
-        float x[8];
-        raw[p].get(x);
+      if (r >= first && r < end) bits = raw[p].top_bits(bits);
+    }
+    float top = Raw8<T>::value(bits);
+    if (!Raw8<T>::finite(bits)) {
+      // NaN and infinities do not set the scale: once more, without them
+      top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float m = fabsf(x[i]);
-          if (m < INFINITY) top = fmaxf(top, m);                // NaN and infinities do not set the scale
+      for (int p = 0; p < kPasses; ++p) {
+        const int r = p * kRows + lane / kLanesPerRow;
+        if (r >= first && r < end) {
+          float x[8];
+          raw[p].get(x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (fabsf(x[i]) < INFINITY) top = fmaxf(top, fabsf(x[i]));
         }
       }
     }
@@ -157,14 +189,41 @@ __device__ __forceinline__ void store8<__half>(__half* p, const float (&y)[8]) {
                                             pack2<false>(y[4], y[5]), pack2<false>(y[6], y[7]));
 }
 
+// What the packed attention kernel needs beside the expanded keys and values (CTA 0), and zeros behind the last query.
+__device__ __forceinline__ void expansion_extras(const Fp8GatherArgs& a) {
+  const long long cta = (static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+  const long long ctas = static_cast<long long>(gridDim.x) * gridDim.y * gridDim.z;
+  const long long words = a.row_bytes / 4;
+  uint32_t* out = static_cast<uint32_t*>(a.out);
+  for (long long i = max(a.cu_q[a.c.n], 0) * words + cta * blockDim.x + threadIdx.x; i < a.tq * words; i += ctas * blockDim.x)
+    out[i] = 0u;
+  if (cta != 0 || threadIdx.x >= 32) return;
+  const int lane = threadIdx.x;
+  int base = 0;
+  if (lane == 0) a.cu_k[0] = 0;
+  for (int i0 = 0; i0 <= a.c.n; i0 += 32) {
+    const int i = i0 + lane;
+    int x = i < a.c.n ? max(a.c.kv_lens[i], 0) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (i < a.c.n) a.cu_k[i + 1] = base + x;
+    if (i <= a.c.n) a.first_row[i] = i * a.pitch;
+    base += __shfl_sync(0xffffffffu, x, 31);
+  }
+}
+
 // One warp per (sequence, 16-token block, K or V, head): codes * scale into a token-major buffer.  Blocks whose page is
-// not held, and the rows from a sequence's end to the next multiple of 128 (zero_to), become zeros.
+// not held, and the rows from a sequence's end to the next multiple of 128 (expansion), become zeros.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
   constexpr int kLanesPerRow = D / 8;
   constexpr int kRows = 32 / kLanesPerRow;
   constexpr int kPasses = kKvBlock / kRows;
   const int lane = threadIdx.x & 31;
+  if (a.off == nullptr) expansion_extras(a);
   const int unit = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (unit >= 2 * a.c.heads) return;
   const bool is_v = unit >= a.c.heads;
@@ -172,15 +231,22 @@ __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
   const int seq = blockIdx.z;
   const int per = a.c.page_size / kKvBlock;
   const int len = a.c.kv_lens[seq];
-  const int off = a.off[seq];
-  const int stop = a.zero_to > 0 ? min((len + 127) / 128 * 128, a.zero_to) : len;
-  if (len < 0 || off < 0 || off + max(stop, len) > a.rows) {
+  const int off = a.off != nullptr ? a.off[seq] : seq * a.pitch;
+  const int stop = a.off == nullptr ? (len + 127) / 128 * 128 : len;
+  if (len < 0 || off < 0 || stop > (a.off == nullptr ? a.pitch : a.rows - off)) {
     if (lane == 0) atomicCAS(a.c.status, 0, kKvStatusPages);
     return;
+  }
+  int unseen_from = 0, unseen_to = 0;   // rows that nobody looks at
+  if (a.off == nullptr && a.window_left >= 0) {
+    const int first_q = len - (a.cu_q[seq + 1] - a.cu_q[seq]);
+    unseen_to = max(first_q - a.window_left, 0) / 128 * 128;
+    unseen_from = min(a.sinks, 0x7fffff00) / 128 * 128 + (a.sinks % 128 != 0 ? 128 : 0);
   }
   T* out = static_cast<T*>(is_v ? a.out_v : a.out_k) + static_cast<long long>(off) * a.c.heads * D + head * D +
            (lane % kLanesPerRow) * 8;
   for (int blk = blockIdx.y; blk * kKvBlock < stop; blk += gridDim.y) {
+    if (blk * kKvBlock >= unseen_from && blk * kKvBlock < unseen_to) continue;
     const int slot = blk / per;
     int page = -1;
     if (blk * kKvBlock < len) {
@@ -331,7 +397,10 @@ cudaError_t fp8_cache_append(const Fp8AppendArgs& a, cudaStream_t s) {
 
 cudaError_t fp8_cache_gather(const Fp8GatherArgs& a, cudaStream_t s) {
   if (!view_ok(a.c)) return cudaErrorInvalidValue;
-  if (a.c.n == 0 || a.rows == 0) return cudaSuccess;
+  if (a.c.n == 0 || (a.rows == 0 && a.off != nullptr)) return cudaSuccess;
+  if (a.off == nullptr && (a.cu_q == nullptr || a.cu_k == nullptr || a.first_row == nullptr || a.out == nullptr || a.row_bytes % 4 != 0 ||
+                           static_cast<long long>(a.pitch) * a.c.n > a.rows))
+    return cudaErrorInvalidValue;
   int blocks = (a.max_kv + 127) / 128 * 8;
   blocks = blocks < 1 ? 1 : (blocks > 65535 ? 65535 : blocks);
   const dim3 grid((2 * a.c.heads + 3) / 4, blocks, a.c.n);

@@ -110,7 +110,7 @@ void fp8_cache_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor
 
 void fp8_cache_gather(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs,
                       const at::Tensor& table, const at::Tensor& kv_lens, const at::Tensor& off, const at::Tensor& out_k,
-                      const at::Tensor& out_v, int64_t zero_to, int64_t max_kv) {
+                      const at::Tensor& out_v, int64_t max_kv) {
   c10::cuda::CUDAGuard guard(k.device());
   teb200::Fp8GatherArgs a;
   a.c = cache_view(k, v, ks, vs, table, kv_lens);
@@ -124,10 +124,47 @@ void fp8_cache_gather(const at::Tensor& k, const at::Tensor& v, const at::Tensor
   TORCH_CHECK(off.numel() >= a.c.n, "offsets: one per sequence");
   a.off = int_vec(off, off.numel(), k.device(), "offsets");
   a.rows = static_cast<int>(out_k.size(0));
-  a.zero_to = static_cast<int>(zero_to);
   a.max_kv = static_cast<int>(max_kv);
   const cudaError_t e = teb200::fp8_cache_gather(a, cur_stream());
   TORCH_CHECK(e == cudaSuccess, "fp8_cache_gather failed: ", cudaGetErrorString(e));
+}
+
+// Keys and values expanded for the packed attention kernel, pitch rows apart: {k, v, out, cumulative lengths, first rows};
+// out has its rows behind the last query zeroed and waits for the others.
+std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
+                                         const at::Tensor& vs, const at::Tensor& table, const at::Tensor& cu_q,
+                                         const at::Tensor& kv_lens, int64_t max_kv, int64_t window_left, int64_t sinks) {
+  c10::cuda::CUDAGuard guard(k.device());
+  teb200::Fp8GatherArgs a;
+  a.c = cache_view(k, v, ks, vs, table, kv_lens);
+  TORCH_CHECK(q.device() == k.device() && q.dim() == 3 && q.size(0) <= INT_MAX && sinks >= 0 && sinks <= INT_MAX &&
+                  window_left <= INT_MAX && max_kv > 0,
+              "attend: a size is out of range, or the queries are on another device than the cache");
+  TORCH_CHECK(q.size(2) == a.c.d && q.size(1) % a.c.heads == 0 && q.size(1) > 0, "queries must be [tokens, heads, ", str(a.c.d),
+              "] with a multiple of the cache's ", str(a.c.heads), " heads");
+  const int64_t pitch = (max_kv + 127) / 128 * 128;
+  TORCH_CHECK(pitch * a.c.n <= INT_MAX, "attend: sequences times max_kv is out of range");
+  const at::Tensor ek = at::empty({pitch * a.c.n, a.c.heads, a.c.d}, q.options());
+  const at::Tensor ev = at::empty_like(ek);
+  const at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  const at::Tensor meta = at::empty({2, a.c.n + 1}, cu_q.options());
+  a.dtype = value_type(q, "queries");
+  a.out_k = ek.data_ptr();
+  a.out_v = ev.data_ptr();
+  a.rows = static_cast<int>(pitch * a.c.n);
+  a.pitch = static_cast<int>(pitch);
+  a.max_kv = static_cast<int>(max_kv);
+  a.cu_q = int_vec(cu_q, a.c.n + 1, k.device(), "cu_q");
+  a.window_left = static_cast<int>(window_left < 0 ? -1 : window_left);
+  a.sinks = static_cast<int>(sinks);
+  a.cu_k = meta.data_ptr<int>();
+  a.first_row = a.cu_k + a.c.n + 1;
+  a.out = out.data_ptr();
+  a.tq = static_cast<int>(q.size(0));
+  a.row_bytes = q.size(1) * q.size(2) * q.element_size();
+  const cudaError_t e = teb200::fp8_cache_gather(a, cur_stream());
+  TORCH_CHECK(e == cudaSuccess, "fp8_cache_expand failed: ", cudaGetErrorString(e));
+  return {ek, ev, out, meta.select(0, 0), meta.select(0, 1)};
 }
 
 at::Tensor fp8_cache_attend(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
@@ -206,6 +243,7 @@ void copy_pages(const std::vector<at::Tensor>& tensors, const at::Tensor& src, c
 void register_kv(py::module_& m) {
   m.def("fp8_cache_append", teb200::traced("teb200.fp8_cache_append", &fp8_cache_append));
   m.def("fp8_cache_gather", teb200::traced("teb200.fp8_cache_gather", &fp8_cache_gather));
+  m.def("fp8_cache_expand", teb200::traced("teb200.fp8_cache_expand", &fp8_cache_expand));
   m.def("fp8_cache_attend", teb200::traced("teb200.fp8_cache_attend", &fp8_cache_attend));
   m.def("copy_pages", teb200::traced("teb200.copy_pages", &copy_pages));
 }

@@ -41,11 +41,21 @@ struct Fp8GatherArgs {
   Fp8CacheView c;
   void* out_k = nullptr;        // [rows, heads, d] contiguous
   void* out_v = nullptr;
-  const int* off = nullptr;     // [n] first row of every sequence
+  const int* off = nullptr;     // [n] first row of every sequence (nullptr: expansion, below)
   int rows = 0;
-  int zero_to = 0;              // > 0: rows up to the next multiple of 128 (at most zero_to rows) are zeroed
   int max_kv = 0;               // longest sequence (sizes the grid, longer ones are handled)
   int dtype = 0;
+  // Expansion for the packed attention kernel: sequence i starts at row i * pitch and is followed by zeros up to the next
+  // multiple of 128 rows; 128-row blocks that no query of the step sees are left out.  The launch also writes what that
+  // kernel needs beside it: cumulative lengths, first rows, and zeros in the output rows behind the last query.
+  int pitch = 0;
+  const int* cu_q = nullptr;    // [n + 1]
+  int window_left = -1, sinks = 0;
+  int* cu_k = nullptr;          // [n + 1]
+  int* first_row = nullptr;     // [n + 1]
+  void* out = nullptr;          // [tq, row_bytes]
+  int tq = 0;
+  long long row_bytes = 0;      // multiple of 4
 };
 cudaError_t fp8_cache_gather(const Fp8GatherArgs& a, cudaStream_t stream);
 

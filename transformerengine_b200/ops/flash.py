@@ -157,11 +157,10 @@ class _FlashVarlenFunc(torch.autograd.Function):
         return (dq, dk, dv) + (None,) * 11
 
 
-def flash_varlen_forward(q, k, v, cu_q, cu_k, off_q, off_k, max_sq, max_sk, scale, causal, window_left, sink_tokens):
-    """Forward only, bottom-right aligned: the attention of prompt chunks over an expanded key/value cache.  Rows of ``q``
-    outside every sequence give zeros."""
+def flash_varlen_forward(q, k, v, out, cu_q, cu_k, off_q, off_k, max_sq, max_sk, scale, causal, window_left, sink_tokens):
+    """Forward only, bottom-right aligned, into ``out``: the attention of prompt chunks over an expanded key/value cache.
+    Rows outside every sequence are not written."""
     C_ = _ext.get()
-    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(cu_q.numel() - 1, q.shape[1], (max_sq + 127) // 128 * 128, dtype=torch.float32, device=q.device)
     C_.flash_fwd_varlen(_thd_view(q), _thd_view(k), _thd_view(v), _thd_view(out), lse, cu_q, cu_k, off_q, off_k, max_sq,
                         max_sk, scale, bool(causal), True, C_.status(q.device.index), window_left=window_left,
