@@ -255,7 +255,9 @@ def run(state):
     if c["kind"] == "pages":
         if own:
             import transformerengine_b200 as te
-            te.kv_cache.copy_pages([x for kind in ("k", "ks", "v", "vs") for x in state[kind].unbind(0)], state["src"], state["dst"])
+            if "layers" not in state:       # a program holds its layers' caches one by one
+                state["layers"] = [te.kv_cache.FP8KVCache(*t) for t in zip(*(state[kind].unbind(0) for kind in ("k", "v", "ks", "vs")))]
+            te.kv_cache.copy_pages(state["layers"], state["src"], state["dst"])
         else:
             src, dst = state["src"].cuda().long(), state["dst"].cuda().long()
             k, v = state["k"].view(torch.uint8), state["v"].view(torch.uint8)
