@@ -176,20 +176,23 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
     ``p - left .. p``, plus the first ``sink_tokens`` tokens; -1 leaves a side open, and the right side is the causal
     one.  ``max_q`` / ``max_kv`` bound the queries and tokens of a sequence.  Rows that see nothing, and rows behind the
     last sequence, are zero.  There is no backward pass."""
-    if torch.is_grad_enabled() and q.requires_grad:
+    if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("attention over the 8-bit cache has no backward pass: call it under torch.no_grad()")
-    left = -1 if window is None else int(window[0])
-    if window is not None and window[1] >= 0 and not (causal and window[1] == 0):
-        raise ValueError("attention over the 8-bit cache takes windows with a left side only (right: -1, or 0 with causal)")
-    if left >= 0 and not causal:
-        raise ValueError("a sliding window over the 8-bit cache needs the causal mask")
+    left = -1
+    if window is not None:
+        left, right = window
+        if right >= 0 and not (causal and right == 0):
+            raise ValueError("attention over the 8-bit cache takes windows with a left side only (right: -1, or 0 with causal)")
+        if left >= 0 and not causal:
+            raise ValueError("a sliding window over the 8-bit cache needs the causal mask")
     if sink_tokens < 0:
         raise ValueError("sink_tokens must not be negative")
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    _, hq, d = q.shape
+    if scale is None:
+        scale = d ** -0.5
     if not _cuda(cache):
         return _attend_ref(q, cache, page_table, cu_q, kv_lens, scale, causal, left, sink_tokens)
-    hq, hk, d = q.shape[1], cache.k.shape[1], q.shape[2]
-    if d == 128 and hq // hk * max_q > _DIRECT_ROWS and max_kv > 0 and q.dtype in (torch.bfloat16, torch.float16):
+    if d == 128 and hq * max_q > _DIRECT_ROWS * cache.k.shape[1] and max_kv > 0 and q.dtype in (torch.bfloat16, torch.float16):
         return _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
     return _ext.get().fp8_cache_attend(q, *cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
 

@@ -84,7 +84,7 @@ def _import(path: str):
 
 
 def available() -> bool:
-    return so_path() is not None
+    return _mod is not None or so_path() is not None   # (the search lists the package's directory: once loaded, no more)
 
 
 def get():
