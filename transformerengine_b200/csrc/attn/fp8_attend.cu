@@ -48,18 +48,6 @@ struct AttendParams {
   int4* cuts;        // [ctas] the cut sequence that the CTA begins: sequence, first row, slot, last CTA; slot < 0: none
 };
 
-#ifndef ST1
-#define ST1 2
-#define CT1 3
-#define ST2 3
-#define CT2 2
-#define ST3 3
-#define CT3 4
-#define ST4 4
-#define CT4 3
-#define ST5 3
-#define CT5 2
-#endif
 template <int D>
 struct Cfg {
   static constexpr int kStep = D == 256 ? 16 : 32;      // tokens per step and warp
@@ -67,10 +55,13 @@ struct Cfg {
   static constexpr int kBlocks = kStep / kKvBlock;
   static constexpr int kLookahead = 32 / kBlocks;       // steps whose pages and scales a warp looks up at once
 };
+// Steps in flight per warp and CTAs per SM: about 192 KB of rings per SM either way.  At d 128 two CTAs with three steps and
+// three with two are alike (64 sequences of up to 8000 tokens: 104 and 107 us, 4 of up to 130000: 145 and 153), steps of
+// 16 tokens are slower (109 - 121 us: the exchanges per step double).  At d 64 a step is half as many bytes.
 template <int D, int NT>
 struct Tune {
-  static constexpr int kStages = D == 64 ? (NT == 1 ? ST3 : ST4) : (D == 128 ? (NT == 1 ? ST1 : ST2) : ST5);
-  static constexpr int kCtas = D == 64 ? (NT == 1 ? CT3 : CT4) : (D == 128 ? (NT == 1 ? CT1 : CT2) : CT5);
+  static constexpr int kStages = D == 64 && NT == 2 ? 4 : 3;
+  static constexpr int kCtas = D == 64 ? (NT == 1 ? 4 : 3) : 2;
   static constexpr int kRing = kWarps * kStages * 2 * Cfg<D>::kStepBytes;
   static constexpr int kParts = kWarps * NT * 8 * (D + 4) * 4;   // the warps' outputs, over the rings
   static constexpr int kSmem = (kRing > kParts ? kRing : kParts) + 128;   // to start on a 128-byte line
@@ -97,6 +88,9 @@ __device__ __forceinline__ uint4 lds16(uint32_t p) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
   return v;
+}
+__device__ __forceinline__ void sts16_zero(uint32_t p) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(p), "r"(0) : "memory");
 }
 __device__ __forceinline__ uint2 lds8(uint32_t p) {
   uint2 v;
@@ -393,24 +387,33 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
     const bool need_mask = !all_held || tok0 + STEP - 1 > hi_min || (tok0 < lo_max && tok0 + STEP > a.sinks);
     uint32_t pf[NT][NB][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float mx[2] = {-INFINITY, -INFINITY};
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const float lv = static_cast<float>(static_cast<int>(__float_as_uint(vs[b]) >> 23) - 127);  // log2 by the exponent
         const float c[2] = {row_scale[t][0] * ks[b], row_scale[t][1] * ks[b]};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = fmaf(s[t][b][e], c[e & 1], lv);
-          if (need_mask) {
+        for (int e = 0; e < 4; ++e) s[t][b][e] = fmaf(s[t][b][e], c[e & 1], lv);
+      }
+    if (need_mask) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
             const int tok = tok0 + b * kKvBlock + g8 + (e >> 1) * 8;
             const bool seen = held[b] && tok <= hi[t][e & 1] && (tok >= lo[t][e & 1] || tok < a.sinks);
-            if (!seen) x = -INFINITY;
+            if (!seen) s[t][b][e] = -INFINITY;
           }
-          s[t][b][e] = x;
-          mx[e & 1] = fmaxf(mx[e & 1], x);
-        }
-      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e & 1] = fmaxf(mx[e & 1], s[t][b][e]);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -448,18 +451,19 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
     // ---- O^T += V^T P^T
     cp_async_wait<2 * kStages - 1>();
     __syncwarp();
+    if (need_mask) {
+      // tokens hidden from all rows meet probability 0, but what their slots hold may be NaN: zeros in their place
+      const uint32_t stage = ring + n % kStages * kStageBytes + kStepBytes;
+      for (int x = lane; x < STEP * (D / 16); x += 32) {
+        const int row = x / (D / 16), tok = tok0 + row;
+        const bool there = NB == 1 ? held[0] : (row < kKvBlock ? held[0] : held[NB - 1]);
+        if (!there || tok > hi_max || (tok < lo_min && tok >= a.sinks)) sts16_zero(stage + place<D>(row, x % (D / 16)));
+      }
+      __syncwarp();
+    }
     constexpr int VP = D >= 128 ? D / 128 : 1;   // pieces of a value row per lane
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      // hidden tokens meet probability 0, but what their slots hold may be NaN
-      bool drop[4] = {false, false, false, false};
-      if (need_mask) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {   // tokens 2c, 2c + 1, 2c + 8, 2c + 9
-          const int tok = tok0 + b * kKvBlock + c4 * 2 + (t & 1) + (t >> 1) * 8;
-          drop[t] = !held[b] || tok > hi_max || (tok < lo_min && tok >= a.sinks);
-        }
-      }
 #pragma unroll
       for (int i = 0; i < VP; ++i) {
         constexpr int kWords = D == 64 ? 2 : 4;
@@ -476,7 +480,6 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
             const uint4 x = lds16(from);
             wv[t][0] = x.x; wv[t][1] = x.y; wv[t][2] = x.z; wv[t][3] = x.w;
           }
-          if (need_mask && drop[t]) wv[t][0] = wv[t][1] = wv[t][2] = wv[t][3] = 0u;
         }
 #pragma unroll
         for (int k = 0; k < kWords; ++k) {
