@@ -173,16 +173,35 @@ def test_attend_matches_64_bits(case):
 @pytest.mark.parametrize("qs,lens,window,sinks", [([100, 300, 1], [700, 300, 129], -1, 0), ([257, 40], [2000, 41], 128, 5),
                                                   ([65, 0, 70], [65, 9, 69], 10, 2), ([130, 20], [1000, 900], 700, 300)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_attend_of_prompt_chunks(qs, lens, window, sinks, dtype):
+@pytest.mark.parametrize("expand", [True, False])
+def test_attend_of_prompt_chunks(qs, lens, window, sinks, dtype, expand, monkeypatch):
+    monkeypatch.setattr(kc, "_expands", lambda *a: expand)
     g = torch.Generator().manual_seed(7)
     cache, table = _filled(lens, 2, 64, 128, g)
     q = torch.randn(sum(qs) + 1, 8, 128, generator=g).to(dtype).cuda()
-    assert 4 * max(qs) > kc._DIRECT_ROWS                                   # the packed 16-bit kernels
     o = kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_q=max(qs), max_kv=max(lens), window=(window, 0), sink_tokens=sinks)
     te.check_status()
     want, mass = _oracle(q, cache, table, qs, lens, window, sinks)
-    _check_attend(o, want, mass, lens, 6.0, torch.finfo(dtype).eps / 2)    # these round the probabilities to the inputs' type
+    # the packed kernels round the probabilities to the inputs' type
+    _check_attend(o, want, mass, lens, 6.0, torch.finfo(dtype).eps / 2 if expand else 2.0 ** -11)
     assert (o[sum(qs):] == 0).all()
+
+
+def test_attend_takes_any_window_and_scale(monkeypatch):
+    """Windows and sinks beyond every length, more queries than tokens, a negative scale."""
+    g = torch.Generator().manual_seed(18)
+    qs, lens = [7, 3], [4, 300]
+    cache, table = _filled(lens, 2, 64, 128, g)
+    q = torch.randn(10, 4, 128, generator=g).to(torch.bfloat16).cuda()
+    kw = dict(max_q=7, max_kv=300)
+    o = kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), window=(2 ** 31 - 1, 0), sink_tokens=2 ** 31 - 1, **kw)
+    assert torch.equal(o, kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), **kw))
+    q = torch.randn(100, 4, 128, generator=g).to(torch.bfloat16).cuda()
+    monkeypatch.setattr(kc, "_expands", lambda *a: True)                     # not taken: they need a positive scale
+    o = kc.attend(q, cache, table, _i32([0, 0, 100]), _i32(lens), max_q=100, max_kv=300, scale=-128 ** -0.5)
+    want, mass = _oracle(-q, cache, table, [0, 100], lens, -1, 0)
+    _check_attend(o, want, mass, lens, 6.0, 2.0 ** -11)
+    te.check_status()
 
 
 def test_attend_without_causal_mask():

@@ -285,6 +285,8 @@ def test_manager_refusals():
         te.InferenceParams(2, 32, cache_dtype=torch.int8, **kw)
     with pytest.raises(ValueError, match="8-bit cache"):
         te.InferenceParams(2, 32, window_size=4, **kw)
+    with pytest.raises(ValueError, match="need a paged cache"):
+        te.InferenceParams(2, 32, **kw).fork_sequence(0, 1)
 
 
 def test_pages_out_of_the_window_return_to_the_pool():

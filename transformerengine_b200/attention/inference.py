@@ -466,20 +466,23 @@ class InferenceParams:
             self.cache_manager.post_step()
             self._pending_post = False
 
+    def _pages(self) -> PagedKVCacheManager:
+        if not isinstance(self.cache_manager, PagedKVCacheManager):
+            raise ValueError("forking, cutting back and compacting need a paged cache")
+        self._complete_step()
+        return self.cache_manager
+
     def fork_sequence(self, seq: int, new_seq: int) -> None:
         """After a step: ``new_seq`` continues from what ``seq`` holds (paged caches; pages are shared until written)."""
-        self._complete_step()
-        self.cache_manager.fork_sequence(seq, new_seq)
+        self._pages().fork_sequence(seq, new_seq)
 
     def truncate_sequence(self, seq: int, length: int) -> None:
         """After a step: cut a sequence back to its first ``length`` tokens (paged caches)."""
-        self._complete_step()
-        self.cache_manager.truncate_sequence(seq, length)
+        self._pages().truncate_sequence(seq, length)
 
     def compact(self) -> int:
         """After a step: move the pages in use to the front of the pool (paged caches); returns how many moved."""
-        self._complete_step()
-        return self.cache_manager.compact()
+        return self._pages().compact()
 
     def get_seqlens_pre_step(self) -> torch.Tensor:
         return torch.tensor(list(self.sequences.values()), dtype=torch.int32)

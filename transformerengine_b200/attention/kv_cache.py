@@ -28,7 +28,8 @@ _MAX_EXP = 60
 
 
 class FP8KVCache(NamedTuple):
-    """The 8-bit cache of one layer (:meth:`allocate` makes an empty one)."""
+    """The 8-bit cache of one layer (:meth:`allocate` makes an empty one, :func:`append` fills it: scales that are not
+    powers of two give wrong results)."""
 
     k: torch.Tensor          # float8_e4m3fn [pages, heads, page_size, d]
     v: torch.Tensor
@@ -161,9 +162,18 @@ def gather(cache: FP8KVCache, page_table: torch.Tensor, kv_lens: torch.Tensor, o
     return k, v
 
 
-# Query rows per key head (queries x heads of a group) from which the codes are expanded once and the packed 16-bit
-# attention kernels take over from the kernel that reads them in place.
-_DIRECT_ROWS = 64
+def _expands(n: int, hq: int, hk: int, max_q: int) -> bool:
+    """Whether expanding the codes once for the packed 16-bit attention kernel beats the kernel that reads them in place.
+
+    The latter walks the cache once for every 16 query rows of a key head (4.3e-5 us per tile and token on all SMs), the
+    former takes 0.02 us per token and wave of its CTAs (256 queries of a head each).  Measured, us in place / expanded,
+    32 / 8 heads: 8 sequences of 8000 tokens, 32 queries 187 / 328, 64 queries 350 / 330, 128 queries 670 / 333; one of
+    100000, 128 queries 985 / 1597; 64 of 2000, 64 queries 790 / 649."""
+    rows = hq // hk * max_q
+    if rows <= 64:
+        return False
+    waves = -(-n * hq * -(-max_q // 256) // 148)
+    return n * hk * -(-rows // 16) > 470 * waves
 
 
 def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, *,
@@ -171,7 +181,7 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
            window: Optional[Tuple[int, int]] = None, sink_tokens: int = 0) -> torch.Tensor:
     """Attention of packed queries ``[t, hq, d]`` (fp16 or bf16) over the cached tokens; returns ``[t, hq, d]``.
 
-    Sequence i's queries are rows ``cu_q[i] .. cu_q[i + 1]`` and, under the causal mask, the LAST tokens of its
+    Sequence i's queries are rows ``cu_q[i] .. cu_q[i + 1]`` (``cu_q[0]`` is 0) and, under the causal mask, the LAST tokens of its
     ``kv_lens[i]`` (bottom-right alignment).  ``window = (left, right)`` limits what the query at position p sees to keys
     ``p - left .. p``, plus the first ``sink_tokens`` tokens; -1 leaves a side open, and the right side is the causal
     one.  ``max_q`` / ``max_kv`` bound the queries and tokens of a sequence.  Rows that see nothing, and rows behind the
@@ -192,7 +202,8 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
         scale = d ** -0.5
     if not _cuda(cache):
         return _attend_ref(q, cache, page_table, cu_q, kv_lens, scale, causal, left, sink_tokens)
-    if d == 128 and hq * max_q > _DIRECT_ROWS * cache.k.shape[1] and max_kv > 0 and q.dtype in (torch.bfloat16, torch.float16):
+    # (the packed kernels take the maximum of the raw scores: a positive scale)
+    if d == 128 and scale > 0.0 and max_kv > 0 and _expands(page_table.shape[0], hq, cache.k.shape[1], max_q):
         return _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
     return _ext.get().fp8_cache_attend(q, *cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
 
@@ -216,7 +227,7 @@ def copy_pages(caches: Sequence[Union[torch.Tensor, FP8KVCache]], src: Union[Seq
             tensors.extend(c)
         else:
             tensors.append(c)
-    src, dst = (torch.as_tensor(x, dtype=torch.int32, device="cpu").contiguous() for x in (src, dst))
+    src, dst = (torch.as_tensor(x, dtype=torch.int64, device="cpu").contiguous() for x in (src, dst))
     if src.dim() != 1 or src.shape != dst.shape:
         raise ValueError("copy_pages: as many source pages as destination pages")
     if not tensors or src.numel() == 0:
@@ -231,5 +242,5 @@ def copy_pages(caches: Sequence[Union[torch.Tensor, FP8KVCache]], src: Union[Seq
     if len(set(d)) != len(d) or set(s) & set(d):
         raise ValueError("copy_pages: a page is written twice, or read and written")
     for t in tensors:
-        raw = t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
-        raw[dst.long()] = raw[src.long()]
+        raw = t.view(torch.uint8) if t.element_size() == 1 else t
+        raw[dst] = raw[src]

@@ -763,7 +763,8 @@ AttendParams plan(const Fp8AttendArgs& a) {
   // behind a window all long sequences are alike: whole ones, if they fill the SMs nearly evenly
   const long long waves = (items + resident - 1) / resident;
   const bool alike = tokens < a.max_kv && items * 4 >= waves * resident * 3;
-  if (steps > kDirectSteps + 1 && !alike && items > 0 && a.max_q > 0) {
+  const bool countable = steps * a.c.n * p.row_tiles <= 0x7fffffff;   // the line's length per key head is an int
+  if (steps > kDirectSteps + 1 && !alike && countable && items > 0 && a.max_q > 0) {
     const long long most = steps * items / kMinShare + 1;
     p.ctas = static_cast<int>(most < resident ? most : resident);
   }

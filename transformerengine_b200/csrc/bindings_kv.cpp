@@ -6,6 +6,7 @@
 #include <teb200/nvtx.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <climits>
 #include <string>
 #include <vector>
@@ -137,8 +138,7 @@ std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& 
   c10::cuda::CUDAGuard guard(k.device());
   teb200::Fp8GatherArgs a;
   a.c = cache_view(k, v, ks, vs, table, kv_lens);
-  TORCH_CHECK(q.device() == k.device() && q.dim() == 3 && q.size(0) <= INT_MAX && sinks >= 0 && sinks <= INT_MAX &&
-                  window_left <= INT_MAX && max_kv > 0,
+  TORCH_CHECK(q.device() == k.device() && q.dim() == 3 && q.size(0) <= INT_MAX && sinks >= 0 && max_kv > 0 && max_kv <= INT_MAX - 128,
               "attend: a size is out of range, or the queries are on another device than the cache");
   TORCH_CHECK(q.size(2) == a.c.d && q.size(1) % a.c.heads == 0 && q.size(1) > 0, "queries must be [tokens, heads, ", str(a.c.d),
               "] with a multiple of the cache's ", str(a.c.heads), " heads");
@@ -155,8 +155,8 @@ std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& 
   a.pitch = static_cast<int>(pitch);
   a.max_kv = static_cast<int>(max_kv);
   a.cu_q = int_vec(cu_q, a.c.n + 1, k.device(), "cu_q");
-  a.window_left = static_cast<int>(window_left < 0 ? -1 : window_left);
-  a.sinks = static_cast<int>(sinks);
+  a.window_left = static_cast<int>(window_left < 0 ? -1 : std::min(window_left, max_kv));   // no key lies further back
+  a.sinks = static_cast<int>(std::min(sinks, max_kv));
   a.cu_k = meta.data_ptr<int>();
   a.first_row = a.cu_k + a.c.n + 1;
   a.out = out.data_ptr();
@@ -177,7 +177,7 @@ at::Tensor fp8_cache_attend(const at::Tensor& q, const at::Tensor& k, const at::
               "queries must be [tokens, heads, ", str(a.c.d), "] with a multiple of the cache's ", str(a.c.heads), " heads");
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "queries must be fp16 or bf16");
   TORCH_CHECK(q.device() == k.device() && q.size(0) <= INT_MAX && max_q <= INT_MAX && max_kv <= INT_MAX && max_q >= 0 &&
-                  max_kv >= 0 && sinks >= 0 && sinks <= INT_MAX && window_left <= INT_MAX,
+                  max_kv >= 0 && sinks >= 0,
               "attend: a size is out of range, or the queries are on another device than the cache");
   const at::Tensor qr = rows16(q);
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
@@ -191,8 +191,8 @@ at::Tensor fp8_cache_attend(const at::Tensor& q, const at::Tensor& k, const at::
   a.max_q = static_cast<int>(max_q);
   a.max_kv = static_cast<int>(max_kv);
   a.causal = causal;
-  a.window_left = static_cast<int>(window_left < 0 ? -1 : window_left);
-  a.sinks = static_cast<int>(sinks);
+  a.window_left = static_cast<int>(window_left < 0 ? -1 : std::min(window_left, max_kv));   // no key lies further back
+  a.sinks = static_cast<int>(std::min(sinks, max_kv));
   a.scale = static_cast<float>(scale);
   const long long need = teb200::fp8_attend_workspace(a);
   at::Tensor part;
@@ -205,12 +205,12 @@ at::Tensor fp8_cache_attend(const at::Tensor& q, const at::Tensor& k, const at::
   return out;
 }
 
-// pages[dst[i]] = pages[src[i]] in every tensor of the list; src / dst are int32 CPU tensors
+// pages[dst[i]] = pages[src[i]] in every tensor of the list; src / dst are int64 CPU tensors
 void copy_pages(const std::vector<at::Tensor>& tensors, const at::Tensor& src, const at::Tensor& dst) {
   if (tensors.empty()) return;
-  TORCH_CHECK(src.device().is_cpu() && dst.device().is_cpu() && src.scalar_type() == at::kInt && dst.scalar_type() == at::kInt &&
+  TORCH_CHECK(src.device().is_cpu() && dst.device().is_cpu() && src.scalar_type() == at::kLong && dst.scalar_type() == at::kLong &&
                   src.is_contiguous() && dst.is_contiguous() && src.dim() == 1 && dst.sizes() == src.sizes(),
-              "page ids must be two int32 CPU tensors of one length");
+              "page ids must be two int64 CPU tensors of one length");
   const at::Device dev = tensors[0].device();
   TORCH_CHECK(dev.is_cuda(), "copy_pages needs CUDA tensors");
   std::vector<teb200::PageCopyTensor> list(tensors.size());
@@ -222,19 +222,23 @@ void copy_pages(const std::vector<at::Tensor>& tensors, const at::Tensor& src, c
     list[i].base = t.data_ptr();
     list[i].page_bytes = t.size(0) > 0 ? static_cast<long long>(t.numel() / t.size(0) * t.element_size()) : 0;
   }
-  const int* s = src.data_ptr<int>();
-  const int* d = dst.data_ptr<int>();
+  const int64_t* s = src.data_ptr<int64_t>();
+  const int64_t* d = dst.data_ptr<int64_t>();
   const int64_t n = src.numel();
+  std::vector<int> ids(2 * static_cast<size_t>(n));
   std::vector<uint8_t> seen(static_cast<size_t>(n > 0 ? pages : 0), 0);
   for (int64_t i = 0; i < n; ++i) {
     TORCH_CHECK_VALUE(s[i] >= 0 && s[i] < pages && d[i] >= 0 && d[i] < pages, "copy_pages: page id out of range at pair ", str(i),
                       " (", str(s[i]), " -> ", str(d[i]), " of ", str(pages), " pages)");
     TORCH_CHECK_VALUE(!seen[d[i]], "copy_pages: page ", str(d[i]), " is written twice");
     seen[d[i]] = 1;
+    ids[i] = static_cast<int>(s[i]);
+    ids[n + i] = static_cast<int>(d[i]);
   }
   for (int64_t i = 0; i < n; ++i) TORCH_CHECK_VALUE(!seen[s[i]], "copy_pages: page ", str(s[i]), " is read and written");
   c10::cuda::CUDAGuard guard(dev);
-  const cudaError_t e = teb200::copy_pages(list.data(), static_cast<int>(list.size()), s, d, static_cast<int>(n), cur_stream());
+  const cudaError_t e = teb200::copy_pages(list.data(), static_cast<int>(list.size()), ids.data(), ids.data() + n,
+                                           static_cast<int>(n), cur_stream());
   TORCH_CHECK(e == cudaSuccess, "copy_pages failed: ", cudaGetErrorString(e));
 }
 

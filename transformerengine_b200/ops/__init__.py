@@ -32,7 +32,7 @@ def check_status(device=None) -> None:
     if code != 0:
         st.zero_()
         names = {1: "producer wait", 2: "MMA wait", 3: "epilogue wait", 4: "peer flag wait", 5: "store wait",
-                 6: "bad argument"}
+                 6: "bad argument", 31: "page table, lengths and key/value cache do not fit each other"}
         raise RuntimeError(f"device kernel reported status {code} ({names.get(code, 'unknown')})")
 
 
