@@ -15,7 +15,8 @@
 // fits fp16 whatever the scales (kept within 2^-60 .. 2^60); sums and accumulators are fp32.
 // The steps of all sequences and heads form one line that the resident CTAs share equally, whatever the lengths: a CTA
 // walks the end of one sequence, whole ones, and the beginning of another, and a second kernel joins the sequences that
-// were cut.  Where no sequence is long (kDirectSteps), a CTA per sequence and head takes it whole.
+// were cut.  Where no sequence is long (kDirectSteps), or a window makes them alike, a CTA per sequence and head takes it
+// whole.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -33,8 +34,12 @@ using namespace kvc;
 
 constexpr int kWarps = 4;
 
-constexpr int kDirectSteps = 16;  // up to here a CTA per sequence and head is faster than cutting and joining
-constexpr int kMinShare = 8;      // fewest steps that are worth a CTA of their own
+// A CTA per sequence and head, without cutting and joining, is faster up to kDirectSteps steps, and up to twice as many
+// where there are CTAs for half the SMs or more (us whole / cut, 32 / 8 heads: 700 tokens 8.1 / 11.9 for 1 sequence, 11.0 /
+// 18.3 for 32; 2000 tokens 16.8 / 12.7 and 25.4 / 32.2).  Fewer than kMinShare steps are not worth a CTA of their own
+// (4, 8 and 16 differ by less than 1 us from 1000 to 8000 tokens).
+constexpr int kDirectSteps = 32;
+constexpr int kMinShare = 8;
 
 struct AttendParams {
   Fp8AttendArgs a;
@@ -578,7 +583,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Tune<D, NT>::kCtas)) attend_kern
   uint8_t* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);  // the warps' rings; then their parts of the output
   __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];
   __shared__ float4 sm_meta[kWarps][Tune<D, NT>::kStages][Cfg<D>::kBlocks];   // of a block: K scale, V scale, held
-  __shared__ int sm_scan[kWarps], sm_at[2];
+  __shared__ int sm_scan[kWarps], sm_at[2], sm_total;
   const Fp8AttendArgs& a = p.a;
   cudaTriggerProgrammaticLaunchCompletion();   // the joining kernel may be launched (it waits for this one's end)
   {
@@ -610,12 +615,13 @@ __global__ void __launch_bounds__(kWarps * 32, (Tune<D, NT>::kCtas)) attend_kern
     const int tile = e / a.c.n;
     return walk_of<STEP>(a, e % a.c.n, tile * R, tile * R + R, p.group, blockIdx.x == 0);
   };
-  int mine = 0;
-  for (int e = threadIdx.x; e < entries; e += kWarps * 32) mine += entry(e).steps;
+  int mine = static_cast<int>(threadIdx.x) < entries ? entry(threadIdx.x).steps : 0;
+  const int own = mine;                        // of the first kWarps * 32 entries
+  for (int e = threadIdx.x + kWarps * 32; e < entries; e += kWarps * 32) mine += entry(e).steps;
   const int upto = block_scan(mine, sm_scan);
-  if (threadIdx.x == kWarps * 32 - 1) sm_at[0] = upto;
+  if (threadIdx.x == kWarps * 32 - 1) sm_total = upto;
   __syncthreads();
-  const int per_head = sm_at[0];               // steps of one key head
+  const int per_head = sm_total;               // steps of one key head
   const long long total = static_cast<long long>(per_head) * a.c.heads;
   const long long even = (total + p.ctas - 1) / p.ctas;
   const long long share = (max(even, static_cast<long long>(kMinShare)) + kWarps - 1) / kWarps * kWarps;
@@ -630,8 +636,11 @@ __global__ void __launch_bounds__(kWarps * 32, (Tune<D, NT>::kCtas)) attend_kern
   // the entry that holds step `rem` of the head
   int e = 0, base = 0;
   for (int e0 = 0; e0 < entries; e0 += kWarps * 32) {
-    const int x = e0 + static_cast<int>(threadIdx.x) < entries ? entry(e0 + threadIdx.x).steps : 0;
-    const int incl = block_scan(x, sm_scan) + base;
+    int x = own, incl = upto;
+    if (entries > kWarps * 32) {               // else the sum above was this scan
+      if (e0 > 0) x = e0 + static_cast<int>(threadIdx.x) < entries ? entry(e0 + threadIdx.x).steps : 0;
+      incl = block_scan(x, sm_scan) + base;
+    }
     if (rem >= incl - x && rem < incl) {
       sm_at[0] = e0 + threadIdx.x;
       sm_at[1] = rem - (incl - x);
@@ -764,7 +773,8 @@ AttendParams plan(const Fp8AttendArgs& a) {
   const long long waves = (items + resident - 1) / resident;
   const bool alike = tokens < a.max_kv && items * 4 >= waves * resident * 3;
   const bool countable = steps * a.c.n * p.row_tiles <= 0x7fffffff;   // the line's length per key head is an int
-  if (steps > kDirectSteps + 1 && !alike && countable && items > 0 && a.max_q > 0) {
+  const bool whole = steps <= (items >= 148 ? 2 : 1) * kDirectSteps + 1;
+  if (!whole && !alike && countable && items > 0 && a.max_q > 0) {
     const long long most = steps * items / kMinShare + 1;
     p.ctas = static_cast<int>(most < resident ? most : resident);
   }
