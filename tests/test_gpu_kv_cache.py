@@ -285,6 +285,67 @@ def test_attend_replays_in_a_graph_and_on_another_stream():
     te.check_status()
 
 
+@pytest.mark.parametrize("n,qn,hq,hk,longest", [(200, 1, 4, 1, 4000), (300, 3, 16, 2, 2500), (3, 40, 8, 1, 9000), (2, 1, 8, 8, 20000)])
+def test_attend_shares_ragged_sequences_over_the_ctas(n, qn, hq, hk, longest):
+    """More sequences than threads, several tiles of rows, sequences cut at any place, among them empty and tiny ones."""
+    g = torch.Generator().manual_seed(n)
+    lens = [int(longest ** x) for x in torch.rand(n, generator=g).tolist()]
+    lens[0], lens[-1], lens[n // 2] = longest, 0, 1
+    qs = [int(x) for x in torch.randint(0, qn + 1, (n,), generator=g)]
+    qs[0] = qn
+    cache, table = _filled(lens, hk, 16, 64, g)
+    q = torch.randn(sum(qs) + 5, hq, 64, generator=g).to(torch.float16).cuda()
+    o = kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_q=qn, max_kv=longest)
+    te.check_status()
+    want, mass = _oracle(q, cache, table, qs, lens, -1, 0)
+    _check_attend(o, want, mass, lens, 6.0, 2.0 ** -11)
+    assert torch.equal(o, kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_q=qn, max_kv=longest))   # no order changes it
+    assert (o[sum(qs):] == 0).all()
+
+
+def test_calls_on_two_streams_do_not_meet():
+    g = torch.Generator().manual_seed(19)
+    a, ta = _filled([9000, 500], 4, 64, 128, g)
+    b, tb = _filled([7000, 8000], 4, 64, 128, g)
+    q = torch.randn(2, 16, 128, generator=g).to(torch.bfloat16).cuda()
+    run = lambda c, t, lens: kc.attend(q, c, t, _i32([0, 1, 2]), _i32(lens), max_q=1, max_kv=9000)  # noqa: E731
+    want = run(a, ta, [9000, 500]), run(b, tb, [7000, 8000])
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(one):
+            x = run(a, ta, [9000, 500])
+        with torch.cuda.stream(two):
+            y = run(b, tb, [7000, 8000])
+        got.append((x, y))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[0]) and torch.equal(y, want[1]) for x, y in got)
+    te.check_status()
+
+
+def test_offsets_beyond_32_bits():
+    """The last pages of a cache of 5 GB of codes: append, attend, gather and copies reach them."""
+    g = torch.Generator().manual_seed(20)
+    big = kc.FP8KVCache.allocate(40000, 8, 128, 128, device="cuda")
+    small = kc.FP8KVCache.allocate(8, 8, 128, 128, device="cuda")
+    x = torch.randn(2, 300, 8, 128, generator=g).to(torch.bfloat16).cuda()
+    q = torch.randn(70, 32, 128, generator=g).to(torch.bfloat16).cuda()
+    outs = []
+    for cache, first in ((big, 39996), (small, 4)):
+        table = _i32([[first + 3, first + 1, first + 2]])
+        kc.append(cache, x[0], x[1], table, _i32([0, 300]), _i32([300]))
+        kc.copy_pages([cache], [first + 1], [first])
+        table[0, 1] = first
+        for rows in (1, 70):
+            outs.append(kc.attend(q[:rows], cache, table, _i32([0, rows]), _i32([300]), max_q=rows, max_kv=300))
+        outs += kc.gather(cache, table, _i32([300]), _i32([0]), 300, torch.float32)
+    half = len(outs) // 2
+    assert all(torch.equal(a, b) for a, b in zip(outs[:half], outs[half:]))
+    assert big.k_scale[:39996].abs().sum() == 0
+    te.check_status()
+
+
 def test_bad_pages_and_lengths_are_reported():
     g = torch.Generator().manual_seed(12)
     cache, table = _filled([100], 2, 64, 128, g)
