@@ -363,45 +363,62 @@ __global__ void __launch_bounds__(256) flash_bwd_join_kernel(const FlashParams p
                                               pack16<BF>(acc[4], acc[5]), pack16<BF>(acc[6], acc[7]));
 }
 
-// delta[b, h, s] = sum_d dO * O, one warp per row
+// delta[b, h, s] = sum_d dO * O.  A warp takes kDeltaRows rows, all of whose loads are in flight at once; rows are numbered
+// with the dimension of the smaller stride fastest, so that neighbouring warps read neighbouring memory (134 MB of O and dO
+// in sbhd layout: 61 us with one row per warp numbered by position, 46 us this way).
+constexpr int kDeltaRows = 4;
 __global__ void flash_delta_kernel(const uint16_t* __restrict__ o, const uint16_t* __restrict__ dout, float* delta,
                                    int b, int h, int s, int s_pad, long long o_sb, long long o_sh, long long o_ss,
-                                   long long d_sb, long long d_sh, long long d_ss, int is_bf16,
+                                   long long d_sb, long long d_sh, long long d_ss, int is_bf16, int heads_first,
                                    const int* __restrict__ cu_q, const int* __restrict__ off_q) {
-  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const long long rows = static_cast<long long>(b) * h * s;
-  if (row >= rows) return;
+  const uint32_t row0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kDeltaRows;
+  const uint32_t rows = static_cast<uint32_t>(b) * h * s;    // 32 bits: 64-bit divisions would take longer than the loads
   const int lane = threadIdx.x & 31;
-  const int si = static_cast<int>(row % s);
-  const int hi = static_cast<int>((row / s) % h);
-  const int bi = static_cast<int>(row / (static_cast<long long>(s) * h));
-  long long tok = si;   // row of the [.., s, d] views
-  long long bo = bi;    // their batch index
-  if (cu_q != nullptr) {  // packed sequences: s is the longest length, the views have one batch entry
-    if (si >= cu_q[bi + 1] - cu_q[bi]) return;
-    tok = off_q[bi] + si;
-    bo = 0;
-  }
-  const uint2 a = *reinterpret_cast<const uint2*>(o + bo * o_sb + hi * o_sh + tok * o_ss + lane * 4);
-  const uint2 g = *reinterpret_cast<const uint2*>(dout + bo * d_sb + hi * d_sh + tok * d_ss + lane * 4);
-  float acc = 0.f;
-  const uint32_t aw[2] = {a.x, a.y}, gw[2] = {g.x, g.y};
+  uint2 a[kDeltaRows], g[kDeltaRows];
+  long long at[kDeltaRows];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float a0, a1, g0, g1;
-    if (is_bf16) {
-      a0 = __uint_as_float(aw[i] << 16); a1 = __uint_as_float(aw[i] & 0xffff0000u);
-      g0 = __uint_as_float(gw[i] << 16); g1 = __uint_as_float(gw[i] & 0xffff0000u);
-    } else {
-      const __half2 ah = *reinterpret_cast<const __half2*>(&aw[i]);
-      const __half2 gh = *reinterpret_cast<const __half2*>(&gw[i]);
-      a0 = __low2float(ah); a1 = __high2float(ah); g0 = __low2float(gh); g1 = __high2float(gh);
+  for (int r = 0; r < kDeltaRows; ++r) {
+    at[r] = -1;
+    const uint32_t row = row0 + r;
+    if (row >= rows) continue;
+    const uint32_t inner = heads_first ? h : s, outer = heads_first ? s : h;
+    const uint32_t up = row / inner, low = row - up * inner;
+    const int bi = static_cast<int>(up / outer);
+    const int mid = static_cast<int>(up - bi * outer);
+    const int si = heads_first ? mid : static_cast<int>(low), hi = heads_first ? static_cast<int>(low) : mid;
+    long long tok = si;   // row of the [.., s, d] views
+    long long bo = bi;    // their batch index
+    if (cu_q != nullptr) {  // packed sequences: s is the longest length, the views have one batch entry
+      if (si >= cu_q[bi + 1] - cu_q[bi]) continue;
+      tok = off_q[bi] + si;
+      bo = 0;
     }
-    acc += a0 * g0 + a1 * g1;
+    at[r] = (static_cast<long long>(bi) * h + hi) * s_pad + si;
+    a[r] = *reinterpret_cast<const uint2*>(o + bo * o_sb + hi * o_sh + tok * o_ss + lane * 4);
+    g[r] = *reinterpret_cast<const uint2*>(dout + bo * d_sb + hi * d_sh + tok * d_ss + lane * 4);
   }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-  if (lane == 0) delta[(static_cast<size_t>(bi) * h + hi) * s_pad + si] = acc;
+  for (int r = 0; r < kDeltaRows; ++r) {
+    if (at[r] < 0) continue;
+    float acc = 0.f;
+    const uint32_t aw[2] = {a[r].x, a[r].y}, gw[2] = {g[r].x, g[r].y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float a0, a1, g0, g1;
+      if (is_bf16) {
+        a0 = __uint_as_float(aw[i] << 16); a1 = __uint_as_float(aw[i] & 0xffff0000u);
+        g0 = __uint_as_float(gw[i] << 16); g1 = __uint_as_float(gw[i] & 0xffff0000u);
+      } else {
+        const __half2 ah = *reinterpret_cast<const __half2*>(&aw[i]);
+        const __half2 gh = *reinterpret_cast<const __half2*>(&gw[i]);
+        a0 = __low2float(ah); a1 = __high2float(ah); g0 = __low2float(gh); g1 = __high2float(gh);
+      }
+      acc += a0 * g0 + a1 * g1;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (lane == 0) delta[at[r]] = acc;
+  }
 }
 
 }  // namespace attn
@@ -513,12 +530,15 @@ cudaError_t flash_bwd_join(const FlashArgs& a, cudaStream_t stream) {
 cudaError_t flash_delta(const FlashArgs& a, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.b) * a.hq * a.sq;
   if (rows == 0) return cudaSuccess;
+  if (rows > 0xffffffffll - 64) return cudaErrorInvalidValue;
   if (a.o_ss % 4 || a.o_sh % 4 || a.o_sb % 4 || a.do_ss % 4 || a.do_sh % 4 || a.do_sb % 4) return cudaErrorInvalidValue;
   const int warps = 8;
-  const unsigned grid = static_cast<unsigned>((rows + warps - 1) / warps);
+  const long long per = static_cast<long long>(warps) * attn::kDeltaRows;
+  const unsigned grid = static_cast<unsigned>((rows + per - 1) / per);
   attn::flash_delta_kernel<<<grid, warps * 32, 0, stream>>>(
       reinterpret_cast<const uint16_t*>(a.out), reinterpret_cast<const uint16_t*>(a.dout), a.delta, a.b, a.hq, a.sq,
-      a.s_pad, a.o_sb, a.o_sh, a.o_ss, a.do_sb, a.do_sh, a.do_ss, a.is_bf16 ? 1 : 0, a.cu_q, a.off_q);
+      a.s_pad, a.o_sb, a.o_sh, a.o_ss, a.do_sb, a.do_sh, a.do_ss, a.is_bf16 ? 1 : 0, a.o_sh < a.o_ss ? 1 : 0, a.cu_q,
+      a.off_q);
   return cudaGetLastError();
 }
 
