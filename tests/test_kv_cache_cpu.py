@@ -363,6 +363,11 @@ def test_variants_without_a_cache_kernel_read_expanded_keys():
         params.pre_step(OrderedDict([(0, 9)]))
         o = attn(q, k, v, inference_params=params)
         torch.testing.assert_close(o, attn(q, k, v), rtol=1e-5, atol=1e-6)     # these keys and values are exact in 8 bits
+        params = te.InferenceParams(1, 64, num_heads_kv=2, head_dim_k=16, dtype=torch.float32, is_paged=True, page_size=16, total_num_pages=4,
+                                    device="cpu", cache_dtype=torch.float8_e4m3fn, window_size=3)
+        params.pre_step(OrderedDict([(0, 9)]))
+        with pytest.raises(ValueError, match="keeps a window"):               # this layer looks at everything
+            attn(q, k, v, inference_params=params)
 
 
 def test_generation_with_forks_and_an_8_bit_cache():

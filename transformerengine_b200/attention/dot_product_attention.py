@@ -144,6 +144,8 @@ class DotProductAttention(torch.nn.Module):
                                           scale=self.softmax_scale, window=window, sink_tokens=self.sink_tokens)
             return out if fp8 is None else fp8.output(out)
         if inference_params is not None:
+            if hasattr(inference_params, "check_window"):
+                inference_params.check_window(self.layer_number, window, self.sink_tokens)
             query_layer, key_layer, value_layer, fmt, mask_type, cu_seqlens_q, cu_seqlens_kv = \
                 inference_params.step(self.layer_number, query_layer, key_layer, value_layer, fmt, mask_type)
         # score_mod(score, tensors) -> score edits the scaled scores; autograd differentiates it, so the

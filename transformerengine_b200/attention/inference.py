@@ -383,13 +383,17 @@ class FP8PagedKVCacheManager(PagedKVCacheManager):
         k, v = _kv.gather(cache, table, lens, cu_kv[:-1], total, new_k.dtype, max_kv=max_kv)
         return k, v, [self.lengths[sid] + n for sid, n in self.step_dict.items()]
 
-    def attend(self, layer_number, q, new_k, new_v, *, scale, causal, window, sink_tokens):
-        """Append the packed new tokens ``[t, h, d]`` and attend: packed output ``[t, hq, d]``."""
+    def check_window(self, layer_number, window, sink_tokens) -> None:
+        """Refuse a layer that looks further back than the pages that are kept."""
         if self.window_size is not None:
             left = -1 if window is None else window[0]
             if left < 0 or left > self.window_size or sink_tokens > self.sink_tokens:
                 raise ValueError(f"the cache keeps a window of {self.window_size} and {self.sink_tokens} sinks; layer {layer_number} "
                                  f"looks at a window of {left} and {sink_tokens}")
+
+    def attend(self, layer_number, q, new_k, new_v, *, scale, causal, window, sink_tokens):
+        """Append the packed new tokens ``[t, h, d]`` and attend: packed output ``[t, hq, d]``."""
+        self.check_window(layer_number, window, sink_tokens)
         cache = self._layer(layer_number)
         table, cu, lens, _, max_new, max_kv, _ = self._step_meta()
         _kv.append(cache, new_k, new_v, table, cu, lens, max_new=max_new)
@@ -550,6 +554,11 @@ class InferenceParams:
         mt = "padding_causal_bottom_right" if "causal" in mask_type else "padding"
         return (qp, kf, vf, "thd", mt, torch.tensor(cu, dtype=torch.int32, device=dev),
                 torch.tensor(cu_kv, dtype=torch.int32, device=dev))
+
+    def check_window(self, layer_number, window, sink_tokens) -> None:
+        """Raise if the layer attends to tokens that the cache has given back (8-bit cache with ``window_size``)."""
+        if hasattr(self.cache_manager, "check_window"):
+            self.cache_manager.check_window(layer_number, window, sink_tokens)
 
     def attends(self) -> bool:
         """Whether the cache itself runs attention (``attend``) instead of handing out keys and values (``step``)."""

@@ -388,8 +388,11 @@ cudaError_t fp8_cache_append(const Fp8AppendArgs& a, cudaStream_t s) {
   if (!view_ok(a.c)) return cudaErrorInvalidValue;
   if (a.c.n == 0 || a.t == 0) return cudaSuccess;
   int blocks = (a.max_new + kKvBlock - 2) / kKvBlock + 1;  // a run may start on a block's last row
+  const int per_block = (2 * a.c.heads + 3) / 4;
+  const long long most = 262144 / (static_cast<long long>(per_block) * a.c.n) + 1;   // (a loose max_new starts no millions of CTAs)
+  if (blocks > most) blocks = static_cast<int>(most);
   if (blocks > 65535) blocks = 65535;
-  const dim3 grid((2 * a.c.heads + 3) / 4, blocks, a.c.n);
+  const dim3 grid(per_block, blocks, a.c.n);
   if (a.dtype == kFloat32) return append_d<float>(a, grid, s);
   if (a.dtype == kFloat16) return append_d<__half>(a, grid, s);
   if (a.dtype == kBFloat16) return append_d<__nv_bfloat16>(a, grid, s);
