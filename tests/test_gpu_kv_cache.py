@@ -149,6 +149,8 @@ CASES = [
     (64, 8, 8, 16, [1, 1], [15, 4097], -1, 0, torch.bfloat16),
     (256, 8, 1, 64, [1, 1, 1], [100, 3000, 1], -1, 0, torch.bfloat16),
     (256, 8, 4, 16, [2, 5], [513, 777], 77, 3, torch.float16),
+    (256, 8, 2, 64, [20, 9], [2000, 300], -1, 0, torch.bfloat16),                     # sixteen rows of a wide head at a time
+    (256, 4, 1, 16, [50, 1, 33], [50, 700, 900], 60, 2, torch.float16),
 ]
 
 

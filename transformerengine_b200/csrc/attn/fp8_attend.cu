@@ -68,9 +68,12 @@ template <int D, int NT>
 struct Tune {
   static constexpr int kStages = D == 64 && NT == 2 ? 4 : 3;
   static constexpr int kCtas = D == 64 ? (NT == 1 ? 4 : 3) : 2;
+  // 16 rows at d 256: the accumulators leave no registers for the queries' fragments
+  static constexpr bool kQueriesInSmem = D == 256 && NT == 2;
   static constexpr int kRing = kWarps * kStages * 2 * Cfg<D>::kStepBytes;
   static constexpr int kParts = kWarps * NT * 8 * (D + 4) * 4;   // the warps' outputs, over the rings
-  static constexpr int kSmem = (kRing > kParts ? kRing : kParts) + 128;   // to start on a 128-byte line
+  static constexpr int kRings = kRing > kParts ? kRing : kParts;
+  static constexpr int kSmem = kRings + (kQueriesInSmem ? NT * (D / 16) * 256 : 0) + 128;   // to start on a 128-byte line
 };
 
 // Byte of 16-byte piece `piece` of row `row` within a step.  A K read takes pieces 4i .. 4i + 3 of rows 2j and 2j + 1 at
@@ -283,7 +286,9 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
   }
 
   // ---- queries: fp16 fragments of row g8 of every 8-row tile, scaled by a power of two
-  uint32_t qf[NT][KC * 4][2];
+  constexpr bool kQS = Tune<D, NT>::kQueriesInSmem;
+  uint32_t qf[kQS ? 1 : NT][kQS ? 1 : KC * 4][2];
+  uint2* q_smem = reinterpret_cast<uint2*>(smem + Tune<D, NT>::kRings);   // [NT][KC * 4][32]
   float row_scale[NT][2];             // of columns 2 c4, 2 c4 + 1: score units (log2)
   int hi[NT][2], lo[NT][2];           // visible tokens of those columns: lo <= j <= hi, or j < sinks
 #pragma unroll
@@ -330,7 +335,9 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const __half2 v = __floats2half2_rn(x[i][k * 4 + h * 2] * down, x[i][k * 4 + h * 2 + 1] * down);
-          qf[t][i * 4 + k][h] = *reinterpret_cast<const uint32_t*>(&v);
+          const uint32_t bits = *reinterpret_cast<const uint32_t*>(&v);
+          if (!kQS) qf[kQS ? 0 : t][kQS ? 0 : i * 4 + k][h] = bits;
+          else if (warp == t) reinterpret_cast<uint32_t*>(q_smem + (t * KC * 4 + i * 4 + k) * 32 + lane)[h] = bits;
         }
 #pragma unroll
     for (int e2 = 0; e2 < 2; ++e2) {
@@ -341,6 +348,8 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
       lo[t][e2] = a.window_left >= 0 ? pos - a.window_left : 0;
     }
   }
+
+  if (kQS) __syncthreads();      // every warp has written its fragments of the queries
 
   int n = 0;
   for (int st = s_begin + warp; st < s_end; st += kWarps, ++n) {
@@ -372,7 +381,12 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
           const uint32_t a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[k]));
           const uint32_t a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(wb[k] >> 16));
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma_f16(s[t][b], a0, a1, a2, a3, qf[t][i * 4 + k][0], qf[t][i * 4 + k][1]);
+          for (int t = 0; t < NT; ++t) {
+            uint2 q;
+            if (kQS) q = lds8(smem_u32(q_smem + (t * KC * 4 + i * 4 + k) * 32 + lane));
+            else q = make_uint2(qf[kQS ? 0 : t][kQS ? 0 : i * 4 + k][0], qf[kQS ? 0 : t][kQS ? 0 : i * 4 + k][1]);
+            mma_f16(s[t][b], a0, a1, a2, a3, q.x, q.y);
+          }
         }
       }
     float ks[NB], vs[NB];
@@ -744,12 +758,14 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p) {
 
 int rows_per_tile(const Fp8AttendArgs& a) {
   const long long rows = static_cast<long long>(a.hq / a.c.heads) * a.max_q;
-  return rows <= 8 || a.c.d == 256 ? 8 : 16;   // d 256: the accumulators of 16 rows do not fit the registers
+  // d 256: 16 rows convert a code for twice as many rows, which long prompts gain from (28 x 285 queries 350 -> 274 us, 1024
+  // queries 235 -> 167), but a step's chain of instructions is longer (16 rows on 4 x 4000 tokens: 25 us, in two tiles 21).
+  // 32 rows at d 64 were slower for few rows (32 rows behind a window: 69 against 58 us) and 6 % faster for prompts: left out.
+  return rows <= 8 || (a.c.d == 256 && rows <= 32) ? 8 : 16;
 }
 
 int resident_ctas(int d, int rows) {
-  const int per_sm = d == 64 ? (rows == 8 ? Tune<64, 1>::kCtas : Tune<64, 2>::kCtas)
-                   : d == 128 ? (rows == 8 ? Tune<128, 1>::kCtas : Tune<128, 2>::kCtas) : Tune<256, 1>::kCtas;
+  const int per_sm = d != 64 ? 2 : (rows == 8 ? Tune<64, 1>::kCtas : Tune<64, 2>::kCtas);
   return per_sm * 148;
 }
 
@@ -851,10 +867,10 @@ cudaError_t fp8_attend(const Fp8AttendArgs& a, cudaStream_t s) {
   if (a.tq == 0) return cudaSuccess;
   const AttendParams p = plan(a);
   if (p.ctas > 0 && a.part == nullptr) return cudaErrorInvalidValue;
-  const bool few = rows_per_tile(a) == 8;
-  if (a.c.d == 64) return few ? launch_t<64, 1>(p, s) : launch_t<64, 2>(p, s);
-  if (a.c.d == 128) return few ? launch_t<128, 1>(p, s) : launch_t<128, 2>(p, s);
-  return launch_t<256, 1>(p, s);
+  const int rows = rows_per_tile(a);
+  if (a.c.d == 64) return rows == 8 ? launch_t<64, 1>(p, s) : launch_t<64, 2>(p, s);
+  if (a.c.d == 128) return rows == 8 ? launch_t<128, 1>(p, s) : launch_t<128, 2>(p, s);
+  return rows == 8 ? launch_t<256, 1>(p, s) : launch_t<256, 2>(p, s);
 }
 
 }  // namespace teb200
