@@ -397,3 +397,15 @@ def test_generation_with_forks_and_an_8_bit_cache():
         logits = model(step, inference_params=params).transpose(0, 1)
     for got, at in ((logits[0, :3], slice(53, 56)), (logits[1], slice(50, 56))):
         assert (got - full[1, at]).norm() / full[1, at].norm() < 2.0 ** -3
+
+
+@pytest.mark.parametrize("family", ["mistral", "gpt", "gemma"])
+def test_generation_example_on_the_8_bit_cache(family):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "generation.py")
+    spec = importlib.util.spec_from_file_location("generation_example", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    out = mod.main(["--family", family, "--cache-8bit", "1", "--batch", "3", "--prompt", "6", "--new-tokens", "4"])
+    assert out.shape == (3, 10)
