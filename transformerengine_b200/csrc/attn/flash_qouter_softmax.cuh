@@ -100,6 +100,16 @@ __device__ __forceinline__ void qouter_softmax_role(const FlashParams& p, uint8_
       lo = 0;
     }
     const auto hidden = [&](int key) { return key > lim || key < lo; };
+    // Visible keys of the 32 columns from `first` on, a bit each: one test per score instead of two comparisons.  The
+    // windowed forward, with three masked blocks of eleven at a window of 1024, gains 5 % (248 -> 236 us); the plain causal
+    // one would lose 2.5 % to spills, the dQ pass neither gains nor loses.
+    constexpr bool kBits = WIN != kNoWindow && MODE == kModeFwd;
+    const auto seen_bits = [&](int first) {
+      const int to = lim - first, from = lo - first;
+      uint32_t m = to < 0 ? 0u : (to >= 31 ? 0xffffffffu : (2u << to) - 1u);
+      if (from > 0) m &= from > 31 ? 0u : 0xffffffffu << from;
+      return m;
+    };
     if (MODE == kModeFwd) {
       // pass 1: block maximum of this thread's columns, 32 at a time
       float mx4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
@@ -109,9 +119,10 @@ __device__ __forceinline__ void qouter_softmax_role(const FlashParams& p, uint8_
         tmem_ld_32x32(col_s + c0, s);
         tmem_ld_wait();
         if (need_mask) {
+          const uint32_t seen = kBits ? seen_bits(kv0 + c0) : 0u;
 #pragma unroll
           for (int c = 0; c < 32; ++c)
-            if (hidden(kv0 + c0 + c)) s[c] = __float_as_uint(NEG_INF);
+            if (kBits ? !(seen & (1u << c)) : hidden(kv0 + c0 + c)) s[c] = __float_as_uint(NEG_INF);
         }
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
@@ -142,13 +153,14 @@ __device__ __forceinline__ void qouter_softmax_role(const FlashParams& p, uint8_
         uint32_t w[16];
         tmem_ld_32x32(col_s + c0, s);
         tmem_ld_wait();
+        const uint32_t seen = kBits && need_mask ? seen_bits(kv0 + c0) : 0u;
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
           float e4[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float x = fmaf(__uint_as_float(s[c + e]), p.scale_log2, -m_eff);
-            if (need_mask && hidden(kv0 + c0 + c + e)) x = NEG_INF;
+            if (need_mask && (kBits ? !(seen & (1u << (c + e))) : hidden(kv0 + c0 + c + e))) x = NEG_INF;
             e4[e] = fast_exp2(x);
             sum4[e] += e4[e];
           }
