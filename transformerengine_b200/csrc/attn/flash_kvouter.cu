@@ -222,6 +222,12 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       // key kv_row is visible to query q iff q >= q_min (and the key exists)
       const int q_min = kv_row < p.sk ? (p.causal ? kv_row - p.causal_off : 0) : 0x7fffffff;
       const int q_max = WIN && !(WIN == kWindowSinks && kv_row < p.n_sink) ? kv_row - p.lo_off : 0x7fffffff;
+      uint32_t seen = 0u;   // windowed kernels: visible queries of this thread's 32 columns, a bit each
+      if (WIN && need_mask) {
+        const int to = min(q_max, p.sq - 1) - (qr + half * 32), from = q_min - (qr + half * 32);
+        seen = to < 0 ? 0u : (to >= 31 ? 0xffffffffu : (2u << to) - 1u);
+        if (from > 0) seen &= from > 31 ? 0u : 0xffffffffu << from;
+      }
       uint32_t wp[16], wd[16];
       {
         uint32_t s[32], dp[32];
@@ -241,7 +247,7 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             float y = x * (__uint_as_float(dp[c + e]) - dl[e]);
             if (need_mask) {
               const int q = qr + half * 32 + c + e;
-              const bool vis = q >= q_min && q <= q_max && q < p.sq;
+              const bool vis = WIN ? (seen & (1u << (c + e))) != 0u : q >= q_min && q <= q_max && q < p.sq;
               x = vis ? x : 0.f;
               y = vis ? y : 0.f;
             }
