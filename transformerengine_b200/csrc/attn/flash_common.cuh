@@ -55,6 +55,7 @@ struct FlashParams {
   // sliding window: with `causal` set, key j is visible to query i when j <= i + causal_off (which
   // includes the right extent win_right) and, when has_lo, j >= i + lo_off
   int win_left, win_right, has_lo, lo_off;
+  void* out_lo;      // forward with sinks: out's rounding remainder, same strides (may be nullptr)
   int n_sink;        // keys j < n_sink are visible left of the window too
   int sink_chunks, sink_len;        // dK/dV pass: parts of the queries of a key block that holds sinks (see FlashArgs)
   float* part_sink;

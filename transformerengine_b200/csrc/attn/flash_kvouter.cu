@@ -373,14 +373,17 @@ __global__ void __launch_bounds__(256) flash_bwd_join_kernel(const FlashParams p
 // with the dimension of the smaller stride fastest, so that neighbouring warps read neighbouring memory (134 MB of O and dO
 // in sbhd layout: 61 us with one row per warp numbered by position, 46 us this way).
 constexpr int kDeltaRows = 4;
-__global__ void flash_delta_kernel(const uint16_t* __restrict__ o, const uint16_t* __restrict__ dout, float* delta,
+// o_lo (same strides as o): what rounding O left over; the softmax gradient subtracts delta from dP, and with few visible
+// keys the two nearly cancel.
+__global__ void flash_delta_kernel(const uint16_t* __restrict__ o, const uint16_t* __restrict__ o_lo,
+                                   const uint16_t* __restrict__ dout, float* delta,
                                    int b, int h, int s, int s_pad, long long o_sb, long long o_sh, long long o_ss,
                                    long long d_sb, long long d_sh, long long d_ss, int is_bf16, int heads_first,
                                    const int* __restrict__ cu_q, const int* __restrict__ off_q) {
   const uint32_t row0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kDeltaRows;
   const uint32_t rows = static_cast<uint32_t>(b) * h * s;    // 32 bits: 64-bit divisions would take longer than the loads
   const int lane = threadIdx.x & 31;
-  uint2 a[kDeltaRows], g[kDeltaRows];
+  uint2 a[kDeltaRows], g[kDeltaRows], rest[kDeltaRows];
   long long at[kDeltaRows];
 #pragma unroll
   for (int r = 0; r < kDeltaRows; ++r) {
@@ -402,6 +405,7 @@ __global__ void flash_delta_kernel(const uint16_t* __restrict__ o, const uint16_
     at[r] = (static_cast<long long>(bi) * h + hi) * s_pad + si;
     a[r] = *reinterpret_cast<const uint2*>(o + bo * o_sb + hi * o_sh + tok * o_ss + lane * 4);
     g[r] = *reinterpret_cast<const uint2*>(dout + bo * d_sb + hi * d_sh + tok * d_ss + lane * 4);
+    if (o_lo != nullptr) rest[r] = *reinterpret_cast<const uint2*>(o_lo + bo * o_sb + hi * o_sh + tok * o_ss + lane * 4);
   }
 #pragma unroll
   for (int r = 0; r < kDeltaRows; ++r) {
@@ -420,6 +424,10 @@ __global__ void flash_delta_kernel(const uint16_t* __restrict__ o, const uint16_
         a0 = __low2float(ah); a1 = __high2float(ah); g0 = __low2float(gh); g1 = __high2float(gh);
       }
       acc += a0 * g0 + a1 * g1;
+      if (o_lo != nullptr) {
+        const uint32_t lw = i == 0 ? rest[r].x : rest[r].y;
+        acc += (is_bf16 ? low16<true>(lw) : low16<false>(lw)) * g0 + (is_bf16 ? high16<true>(lw) : high16<false>(lw)) * g1;
+      }
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
@@ -542,7 +550,8 @@ cudaError_t flash_delta(const FlashArgs& a, cudaStream_t stream) {
   const long long per = static_cast<long long>(warps) * attn::kDeltaRows;
   const unsigned grid = static_cast<unsigned>((rows + per - 1) / per);
   attn::flash_delta_kernel<<<grid, warps * 32, 0, stream>>>(
-      reinterpret_cast<const uint16_t*>(a.out), reinterpret_cast<const uint16_t*>(a.dout), a.delta, a.b, a.hq, a.sq,
+      reinterpret_cast<const uint16_t*>(a.out), reinterpret_cast<const uint16_t*>(a.out_lo),
+      reinterpret_cast<const uint16_t*>(a.dout), a.delta, a.b, a.hq, a.sq,
       a.s_pad, a.o_sb, a.o_sh, a.o_ss, a.do_sb, a.do_sh, a.do_ss, a.is_bf16 ? 1 : 0, a.o_sh < a.o_ss ? 1 : 0, a.cu_q,
       a.off_q);
   return cudaGetLastError();

@@ -97,6 +97,8 @@ flash_qouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   const int b = blockIdx.y;
   const SeqView sv = localize(p, b);
   p.out = reinterpret_cast<uint16_t*>(p.out) + static_cast<long long>(sv.q_off) * p.o_ss;
+  if (WIN == kWindowSinks && p.out_lo != nullptr)
+    p.out_lo = reinterpret_cast<uint16_t*>(p.out_lo) + static_cast<long long>(sv.q_off) * p.o_ss;
   const int hk = h / (p.hq / p.hk);
   // first query row of the CTA's two tiles: neighbours, or (few CTAs, causal mask) tile i with tile
   // last - i, so that every CTA walks the same number of key blocks in total
@@ -340,9 +342,9 @@ static cudaError_t launch_qouter(const FlashArgs& a, cudaStream_t stream) {
   p.scale = a.scale;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.is_bf16 = bf ? 1 : 0;
-  if (MODE == kFwd) { p.out = a.out; p.o_sb = a.o_sb; p.o_sh = a.o_sh; p.o_ss = a.o_ss; }
+  if (MODE == kFwd) { p.out = a.out; p.out_lo = a.out_lo; p.o_sb = a.o_sb; p.o_sh = a.o_sh; p.o_ss = a.o_ss; }
   else { p.out = a.dq; p.o_sb = a.dq_sb; p.o_sh = a.dq_sh; p.o_ss = a.dq_ss; }
-  if ((reinterpret_cast<uintptr_t>(p.out) & 15) || p.o_sb % 8 || p.o_sh % 8 || p.o_ss % 8) return cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(p.out) & 15) || (reinterpret_cast<uintptr_t>(p.out_lo) & 15) || p.o_sb % 8 || p.o_sh % 8 || p.o_ss % 8) return cudaErrorInvalidValue;
   p.lse = a.lse; p.delta = a.delta; p.s_pad = a.s_pad; p.status = a.status; p.timeline = a.timeline;
   p.cu_q = a.cu_q; p.cu_k = a.cu_k; p.off_q = a.off_q; p.off_k = a.off_k;
   p.gsplit = 1; p.o_sg = 0;

@@ -15,6 +15,16 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   return BF ? pack_bf16x2(a, b) : pack_f16x2(a, b);
 }
 
+// the two values of a packed word
+template <bool BF>
+__device__ __forceinline__ float low16(uint32_t w) {
+  return BF ? __uint_as_float(w << 16) : __low2float(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF>
+__device__ __forceinline__ float high16(uint32_t w) {
+  return BF ? __uint_as_float(w & 0xffff0000u) : __high2float(*reinterpret_cast<const __half2*>(&w));
+}
+
 // 16 packed words = 32 values = chunks [4*half, 4*half+4) of row r in a [128 x 64] swizzled tile
 __device__ __forceinline__ void store_half_row_sw128(uint8_t* tile, int r, int half, const uint32_t (&w)[16]) {
   uint8_t* row = tile + r * 128;
@@ -238,28 +248,56 @@ __device__ __forceinline__ void qouter_softmax_role(const FlashParams& p, uint8_
   ok = __all_sync(0xffffffffu, ok);
   if (!ok) return;
   const bool row_ok = q_row < p.sq;
-  uint16_t* orow = reinterpret_cast<uint16_t*>(p.out) + b * p.o_sb + h * p.o_sh + static_cast<long long>(q_row) * p.o_ss +
-                   half * 64;
   const float mul = MODE == kModeFwd ? (l_row > 0.f ? 1.f / l_row : 0.f) : p.scale;
+  // A thread holds half a row: the warp's 32 half rows pass through its part of the tile's Q buffer (all score products are
+  // done), so that 8 lanes write a row's 128 bytes at once.  Pieces are exchanged by the row's low bits against conflicts.
+  const uint32_t stage = smem_u32(smem + t * 32768 + wi * 4096);
+  const int first_row = q0 + t * 128 + quarter * 32;
+  const auto write_out = [&](void* to, bool remainder) {
 #pragma unroll 1
-  for (int c0 = 0; c0 < 64; c0 += 32) {
-    uint32_t o[32];
-    if (nt > 0) {
+    for (int c0 = 0; c0 < 64; c0 += 32) {
+      uint32_t o[32];
       tmem_ld_32x32(lane_base + C::kColO + t * 128 + half * 64 + c0, o);
       tmem_ld_wait();
-    } else {
-#pragma unroll
-      for (int c = 0; c < 32; ++c) o[c] = 0u;
-    }
-    if (row_ok) {
 #pragma unroll
       for (int c = 0; c < 32; c += 8) {
         uint32_t q4[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          q4[i] = pack16<BF>(__uint_as_float(o[c + 2 * i]) * mul, __uint_as_float(o[c + 2 * i + 1]) * mul);
-        *reinterpret_cast<uint4*>(orow + c0 + c) = make_uint4(q4[0], q4[1], q4[2], q4[3]);
+        for (int i = 0; i < 4; ++i) {
+          const float x = __uint_as_float(o[c + 2 * i]) * mul, y = __uint_as_float(o[c + 2 * i + 1]) * mul;
+          q4[i] = pack16<BF>(x, y);
+          if (remainder) q4[i] = pack16<BF>(x - low16<BF>(q4[i]), y - high16<BF>(q4[i]));
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((((c0 + c) >> 3) ^ (lane & 7)) << 4)),
+                     "r"(q4[0]), "r"(q4[1]), "r"(q4[2]), "r"(q4[3])
+                     : "memory");
       }
+    }
+    __syncwarp();
+    uint16_t* base = reinterpret_cast<uint16_t*>(to) + b * p.o_sb + h * p.o_sh + half * 64 + (lane & 7) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = i * 4 + (lane >> 3);
+      uint4 v;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "r"(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4))
+                   : "memory");
+      if (first_row + row < p.sq) *reinterpret_cast<uint4*>(base + static_cast<long long>(first_row + row) * p.o_ss) = v;
+    }
+    __syncwarp();
+  };
+  if (nt > 0) {
+    write_out(p.out, false);
+    if (WIN == kWindowSinks && MODE == kModeFwd && p.out_lo != nullptr) write_out(p.out_lo, true);
+  } else if (row_ok) {
+    // no key block at all: zeros (the Q buffer may still be receiving its tile)
+    const long long at = b * p.o_sb + h * p.o_sh + static_cast<long long>(q_row) * p.o_ss + half * 64;
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 8) {
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + at + c) = make_uint4(0u, 0u, 0u, 0u);
+      if (WIN == kWindowSinks && MODE == kModeFwd && p.out_lo != nullptr)
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out_lo) + at + c) = make_uint4(0u, 0u, 0u, 0u);
     }
   }
   if (MODE == kModeFwd && row_ok && half == 0) {

@@ -154,13 +154,24 @@ teb200::FlashArgs flash_args(const at::Tensor& q, const at::Tensor& k, const at:
   return a;
 }
 
+// The rounding remainder of the output (attention with sinks): a tensor like the output.
+void set_out_lo(teb200::FlashArgs& a, const at::Tensor& out, const OptT& out_lo) {
+  if (!out_lo.has_value() || !out_lo->defined()) return;
+  TORCH_CHECK(out_lo->sizes() == out.sizes() && out_lo->strides() == out.strides() && out_lo->scalar_type() == out.scalar_type() &&
+                  out_lo->device() == out.device(),
+              "out_lo must be laid out like the output");
+  a.out_lo = out_lo->data_ptr();
+}
+
 void flash_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
                const at::Tensor& lse, double scale, bool causal, bool bottom_right, const at::Tensor& status,
-               const OptT& timeline, int64_t window_left, int64_t window_right, int64_t sink_tokens) {
+               const OptT& timeline, int64_t window_left, int64_t window_right, int64_t sink_tokens,
+               const OptT& out_lo) {
   c10::cuda::CUDAGuard guard(q.device());
   teb200::FlashArgs a = flash_args(q, k, v, out, lse, scale, causal, bottom_right, status);
   a.window_left = static_cast<int>(window_left); a.window_right = static_cast<int>(window_right);
   a.sink_tokens = static_cast<int>(sink_tokens);
+  set_out_lo(a, out, out_lo);
   if (timeline.has_value() && timeline->defined()) {
     TORCH_CHECK(timeline->scalar_type() == at::kLong && timeline->numel() >= 1024, "timeline must be int64 [64, 16]");
     a.timeline = reinterpret_cast<long long*>(timeline->data_ptr());
@@ -216,11 +227,13 @@ void run_dkdv(teb200::FlashArgs& a, const at::Tensor& k, const at::Tensor& dk, c
 void flash_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                const at::Tensor& out, const at::Tensor& lse, const at::Tensor& delta, const at::Tensor& dq,
                const at::Tensor& dk, const at::Tensor& dv, double scale, bool causal, bool bottom_right,
-               const at::Tensor& status, int64_t window_left, int64_t window_right, int64_t sink_tokens) {
+               const at::Tensor& status, int64_t window_left, int64_t window_right, int64_t sink_tokens,
+               const OptT& out_lo) {
   c10::cuda::CUDAGuard guard(q.device());
   teb200::FlashArgs a = flash_args(q, k, v, out, lse, scale, causal, bottom_right, status);
   a.window_left = static_cast<int>(window_left); a.window_right = static_cast<int>(window_right);
   a.sink_tokens = static_cast<int>(sink_tokens);
+  set_out_lo(a, out, out_lo);
   a.dout = dout.data_ptr();
   a.delta = delta.data_ptr<float>();
   a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
@@ -254,11 +267,13 @@ void set_varlen(teb200::FlashArgs& a, const at::Tensor& q, const at::Tensor& k, 
 void flash_fwd_varlen(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
                       const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k, const at::Tensor& off_q,
                       const at::Tensor& off_k, int64_t max_sq, int64_t max_sk, double scale, bool causal,
-                      bool bottom_right, const at::Tensor& status, int64_t window_left, int64_t window_right, int64_t sink_tokens) {
+                      bool bottom_right, const at::Tensor& status, int64_t window_left, int64_t window_right, int64_t sink_tokens,
+               const OptT& out_lo) {
   c10::cuda::CUDAGuard guard(q.device());
   teb200::FlashArgs a = flash_args(q, k, v, out, lse, scale, causal, bottom_right, status);
   a.window_left = static_cast<int>(window_left); a.window_right = static_cast<int>(window_right);
   a.sink_tokens = static_cast<int>(sink_tokens);
+  set_out_lo(a, out, out_lo);
   set_varlen(a, q, k, cu_q, cu_k, off_q, off_k, max_sq, max_sk);
   TORCH_CHECK(lse.size(0) == a.b && lse.size(1) == a.hq && lse.size(2) >= max_sq, "lse must be [sequences, hq, >= max_sq]");
   cudaError_t e = teb200::flash_fwd(a, cur_stream());
@@ -270,11 +285,13 @@ void flash_bwd_varlen(const at::Tensor& dout, const at::Tensor& q, const at::Ten
                       const at::Tensor& dk, const at::Tensor& dv, const at::Tensor& cu_q, const at::Tensor& cu_k,
                       const at::Tensor& off_q, const at::Tensor& off_k, int64_t max_sq, int64_t max_sk, double scale,
                       bool causal, bool bottom_right, const at::Tensor& status, int64_t window_left,
-                      int64_t window_right, int64_t sink_tokens) {
+                      int64_t window_right, int64_t sink_tokens,
+               const OptT& out_lo) {
   c10::cuda::CUDAGuard guard(q.device());
   teb200::FlashArgs a = flash_args(q, k, v, out, lse, scale, causal, bottom_right, status);
   a.window_left = static_cast<int>(window_left); a.window_right = static_cast<int>(window_right);
   a.sink_tokens = static_cast<int>(sink_tokens);
+  set_out_lo(a, out, out_lo);
   set_varlen(a, q, k, cu_q, cu_k, off_q, off_k, max_sq, max_sk);
   TORCH_CHECK(lse.size(0) == a.b && lse.size(2) % 128 == 0 && lse.size(2) >= max_sq && delta.sizes() == lse.sizes(),
               "lse / delta must be [sequences, hq, s_pad] with s_pad a multiple of 128");
@@ -906,11 +923,11 @@ void register_extra(py::module_& m) {
         py::arg("out_all_ptrs") = std::vector<int64_t>(), py::arg("ar_flag_ptrs") = std::vector<int64_t>());
   m.def("flash_fwd", teb200::traced("teb200.flash_fwd", &flash_fwd), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"),
         py::arg("scale"), py::arg("causal"), py::arg("bottom_right"), py::arg("status"),
-        py::arg("timeline") = py::none(), py::arg("window_left") = -1, py::arg("window_right") = -1, py::arg("sink_tokens") = 0);
+        py::arg("timeline") = py::none(), py::arg("window_left") = -1, py::arg("window_right") = -1, py::arg("sink_tokens") = 0, py::arg("out_lo") = py::none());
   m.def("flash_bwd", teb200::traced("teb200.flash_bwd", &flash_bwd), py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"),
         py::arg("lse"), py::arg("delta"), py::arg("dq"), py::arg("dk"), py::arg("dv"), py::arg("scale"),
         py::arg("causal"), py::arg("bottom_right"), py::arg("status"), py::arg("window_left") = -1,
-        py::arg("window_right") = -1, py::arg("sink_tokens") = 0);
+        py::arg("window_right") = -1, py::arg("sink_tokens") = 0, py::arg("out_lo") = py::none());
   m.def("thd_get_partitioned_indices", teb200::traced("teb200.thd_get_partitioned_indices", &thd_get_partitioned_indices));
   m.def("thd_read_half_tensor", teb200::traced("teb200.thd_read_half_tensor", &thd_read_half_tensor));
   m.def("thd_second_half_lse_correction", teb200::traced("teb200.thd_second_half_lse_correction", &thd_second_half_lse_correction));
@@ -923,11 +940,11 @@ void register_extra(py::module_& m) {
   m.def("flash_fwd_varlen", teb200::traced("teb200.flash_fwd_varlen", &flash_fwd_varlen), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"),
         py::arg("lse"), py::arg("cu_q"), py::arg("cu_k"), py::arg("off_q"), py::arg("off_k"), py::arg("max_sq"),
         py::arg("max_sk"), py::arg("scale"), py::arg("causal"), py::arg("bottom_right"), py::arg("status"),
-        py::arg("window_left") = -1, py::arg("window_right") = -1, py::arg("sink_tokens") = 0);
+        py::arg("window_left") = -1, py::arg("window_right") = -1, py::arg("sink_tokens") = 0, py::arg("out_lo") = py::none());
   m.def("flash_bwd_varlen", teb200::traced("teb200.flash_bwd_varlen", &flash_bwd_varlen), py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"),
         py::arg("out"), py::arg("lse"), py::arg("delta"), py::arg("dq"), py::arg("dk"), py::arg("dv"), py::arg("cu_q"),
         py::arg("cu_k"), py::arg("off_q"), py::arg("off_k"), py::arg("max_sq"), py::arg("max_sk"), py::arg("scale"),
         py::arg("causal"), py::arg("bottom_right"), py::arg("status"), py::arg("window_left") = -1,
-        py::arg("window_right") = -1, py::arg("sink_tokens") = 0);
+        py::arg("window_right") = -1, py::arg("sink_tokens") = 0, py::arg("out_lo") = py::none());
 }
 

@@ -101,6 +101,9 @@ struct FlashArgs {
   int window_left = -1, window_right = -1;
   // Left of the window the first sink_tokens keys stay visible (0: none; only read with window_left >= 0).
   int sink_tokens = 0;
+  // With sinks: what rounding `out` to 16 bits left over, in 16 bits, same strides (nullptr: not kept).  The forward writes
+  // it and the delta pass adds it in, so that delta = rowsum(dO * O) is that of the unrounded output.
+  void* out_lo = nullptr;
   // dK/dV pass with sinks: every query sees the key blocks that hold them, so their queries are split over sink_chunks
   // CTAs of sink_len 64-row blocks.  These CTAs, and all of them with gsplit > 1, leave fp32 partial sums
   // [part][b][hk][rows][dK 128, dV 128] that flash_bwd_join adds and rounds once.

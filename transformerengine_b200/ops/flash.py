@@ -52,16 +52,18 @@ class _FlashFunc(torch.autograd.Function):
         lse = torch.empty(b, h, s_pad, dtype=torch.float32, device=q.device)
         sc = float(scale) if scale is not None else d ** -0.5
         wl, wr = (-1, -1) if window is None else (int(window[0]), int(window[1]))
+        # with sinks the backward also gets what rounding the output left over
+        lo = torch.empty_like(out) if sink_tokens and any(ctx.needs_input_grad[:3]) else None
         C_.flash_fwd(q, k, v, out, lse, sc, bool(causal), bool(bottom_right), C_.status(q.device.index),
-                     window_left=wl, window_right=wr, sink_tokens=sink_tokens)
-        ctx.save_for_backward(q, k, v, out, lse)
+                     window_left=wl, window_right=wr, sink_tokens=sink_tokens, out_lo=lo)
+        ctx.save_for_backward(q, k, v, out, lse, lo)
         ctx.cfg = (sc, bool(causal), bool(bottom_right), wl, wr, sink_tokens)
         return out
 
     @staticmethod
     def backward(ctx, dout):  # type: ignore[override]
         C_ = _ext.get()
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, lo = ctx.saved_tensors
         sc, causal, bottom_right, wl, wr, sink_tokens = ctx.cfg
         dout = _prep(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
@@ -69,7 +71,7 @@ class _FlashFunc(torch.autograd.Function):
             dv = torch.empty_strided(dk.shape, dk.stride(), dtype=dk.dtype, device=dk.device)
         delta = torch.empty_like(lse)
         C_.flash_bwd(dout, q, k, v, out, lse, delta, dq, dk, dv, sc, causal, bottom_right,
-                     C_.status(q.device.index), window_left=wl, window_right=wr, sink_tokens=sink_tokens)
+                     C_.status(q.device.index), window_left=wl, window_right=wr, sink_tokens=sink_tokens, out_lo=lo)
         return dq, dk, dv, None, None, None, None, None, None
 
 
@@ -134,18 +136,19 @@ class _FlashVarlenFunc(torch.autograd.Function):
         lse = torch.empty(nseq, hq, s_pad, dtype=torch.float32, device=q.device)
         sc = float(scale) if scale is not None else d ** -0.5
         qv, kv, vv = _thd_view(q), _thd_view(k), _thd_view(v)
+        lo = torch.empty_like(out) if sink_tokens and any(ctx.needs_input_grad[:3]) else None
         wl, wr = (-1, -1) if window is None else (int(window[0]), int(window[1]))
         C_.flash_fwd_varlen(qv, kv, vv, _thd_view(out), lse, cu_q, cu_k, off_q, off_k, max_sq, max_sk, sc,
                             bool(causal), bool(bottom_right), C_.status(q.device.index), window_left=wl,
-                            window_right=wr, sink_tokens=sink_tokens)
-        ctx.save_for_backward(qv, kv, vv, out, lse, cu_q, cu_k, off_q, off_k)
+                            window_right=wr, sink_tokens=sink_tokens, out_lo=None if lo is None else _thd_view(lo))
+        ctx.save_for_backward(qv, kv, vv, out, lse, cu_q, cu_k, off_q, off_k, lo)
         ctx.cfg = (sc, bool(causal), bool(bottom_right), max_sq, max_sk, wl, wr, sink_tokens)
         return out
 
     @staticmethod
     def backward(ctx, dout):  # type: ignore[override]
         C_ = _ext.get()
-        qv, kv, vv, out, lse, cu_q, cu_k, off_q, off_k = ctx.saved_tensors
+        qv, kv, vv, out, lse, cu_q, cu_k, off_q, off_k, lo = ctx.saved_tensors
         sc, causal, bottom_right, max_sq, max_sk, wl, wr, sink_tokens = ctx.cfg
         dq = torch.zeros(qv.shape[2], qv.shape[1], 128, dtype=qv.dtype, device=qv.device)
         dk = torch.zeros(kv.shape[2], kv.shape[1], 128, dtype=qv.dtype, device=qv.device)
@@ -153,7 +156,8 @@ class _FlashVarlenFunc(torch.autograd.Function):
         delta = torch.empty_like(lse)
         C_.flash_bwd_varlen(_thd_view(dout), qv, kv, vv, _thd_view(out), lse, delta, _thd_view(dq), _thd_view(dk),
                             _thd_view(dv), cu_q, cu_k, off_q, off_k, max_sq, max_sk, sc, causal, bottom_right,
-                            C_.status(qv.device.index), window_left=wl, window_right=wr, sink_tokens=sink_tokens)
+                            C_.status(qv.device.index), window_left=wl, window_right=wr, sink_tokens=sink_tokens,
+                            out_lo=None if lo is None else _thd_view(lo))
         return (dq, dk, dv) + (None,) * 11
 
 
