@@ -287,6 +287,11 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                        static_cast<long long>(kv_row) * p.o_ss + half * 64;
       const float mul = u == 0 ? p.scale : 1.f;
       const uint32_t col0 = (u == 0 ? C::kColDk : C::kColDv) + half * 64;
+      // A thread holds half a row: the warp's 32 half rows pass through its 4 KB of the K and V tiles (all products are
+      // done), so that 8 lanes write a row's 128 bytes at once.  Pieces are exchanged by the row's low bits.  (With sinks
+      // 677 -> 662 us for the backward at a window of 1024; the other instances lose more to spills than they gain.)
+      constexpr bool kStaged = WIN == kWindowSinks;
+      const uint32_t stage = smem_u32(smem) + (warp - 2) * 4096;
       float* part = nullptr;
       if (WIN == kWindowSinks && (sink_block ? p.part_sink : p.part_rest) != nullptr) {
         const int edge = (p_launch.n_sink + 127) / 128 * 128;   // rows in sink blocks
@@ -314,6 +319,17 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                   make_float4(__uint_as_float(o[c]) * mul, __uint_as_float(o[c + 1]) * mul, __uint_as_float(o[c + 2]) * mul,
                               __uint_as_float(o[c + 3]) * mul);
           }
+        } else if (kStaged && N > 0) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            uint32_t q4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              q4[i] = pack16<BF>(__uint_as_float(o[c + 2 * i]) * mul, __uint_as_float(o[c + 2 * i + 1]) * mul);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((((c0 + c) >> 3) ^ (lane & 7)) << 4)),
+                         "r"(q4[0]), "r"(q4[1]), "r"(q4[2]), "r"(q4[3])
+                         : "memory");
+          }
         } else if (row_ok) {
 #pragma unroll
           for (int c = 0; c < 32; c += 8) {
@@ -323,6 +339,21 @@ flash_kvouter_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
               q4[i] = pack16<BF>(__uint_as_float(o[c + 2 * i]) * mul, __uint_as_float(o[c + 2 * i + 1]) * mul);
             *reinterpret_cast<uint4*>(orow + c0 + c) = make_uint4(q4[0], q4[1], q4[2], q4[3]);
           }
+        }
+      }
+      if (kStaged && N > 0 && part == nullptr) {
+        __syncwarp();
+        uint16_t* base = reinterpret_cast<uint16_t*>(u == 0 ? p.out : p.out2) + b * p.o_sb + hk * p.o_sh + half * 64 + (lane & 7) * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = i * 4 + (lane >> 3);
+          uint4 v;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4))
+                       : "memory");
+          const int key = kv0 + quarter * 32 + row;
+          if (key < p.sk) *reinterpret_cast<uint4*>(base + static_cast<long long>(key) * p.o_ss) = v;
         }
       }
     }
