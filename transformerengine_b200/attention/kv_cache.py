@@ -211,8 +211,9 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
 def _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens):
     """Codes expanded to 16 bits (every sequence padded to whole 128-token blocks with zeros), then the packed attention
     kernel: prompt chunks are bound by its products, not by the cache."""
-    k, v, out, cu_k, first = _ext.get().fp8_cache_expand(q, *cache, page_table, cu_q, kv_lens, max_kv, left, sink_tokens)
-    return _flash.flash_varlen_forward(q, k, v, out, cu_q, cu_k, cu_q, first, max_q, max_kv, scale, causal, left, sink_tokens)
+    k, v, out, cu_k, first_k, cut_q, first_q = _ext.get().fp8_cache_expand(q, *cache, page_table, cu_q, kv_lens, max_q, max_kv, left,
+                                                                           sink_tokens)
+    return _flash.flash_varlen_forward(q, k, v, out, cut_q, cu_k, first_q, first_k, max_q, max_kv, scale, causal, left, sink_tokens)
 
 
 def copy_pages(caches: Sequence[Union[torch.Tensor, FP8KVCache]], src: Union[Sequence[int], torch.Tensor],

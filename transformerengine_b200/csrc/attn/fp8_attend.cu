@@ -139,18 +139,12 @@ struct Walk {
 
 template <int STEP>
 __device__ __forceinline__ Walk walk_of(const Fp8AttendArgs& a, int seq, int r0, int r1, int group, bool report) {
+  const SeqFit f = fit_sequence(a.cu_q, a.c.kv_lens, seq, a.tq, a.max_q, a.max_kv);
+  if (f.bad && report) atomicCAS(a.c.status, 0, kKvStatusPages);
   Walk w;
-  w.q_row0 = a.cu_q[seq];
-  w.qlen = a.cu_q[seq + 1] - w.q_row0;
-  w.len = a.c.kv_lens[seq];
-  bool bad = w.q_row0 < 0 || w.q_row0 > a.tq || w.qlen < 0 || w.qlen > a.max_q || w.qlen > a.tq - w.q_row0 || w.len < 0 ||
-             w.len > a.max_kv;
-  if (bad) {
-    if (report) atomicCAS(a.c.status, 0, kKvStatusPages);
-    w.q_row0 = min(max(w.q_row0, 0), a.tq);
-    w.qlen = min(min(max(w.qlen, 0), a.max_q), a.tq - w.q_row0);
-    w.len = min(max(w.len, 0), a.max_kv);
-  }
+  w.q_row0 = f.q_row0;
+  w.qlen = f.qlen;
+  w.len = f.len;
   w.sink_steps = 0;
   w.gap = 0;
   const int rows = min(r1, w.qlen * group);

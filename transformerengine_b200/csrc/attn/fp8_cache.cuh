@@ -9,6 +9,26 @@
 namespace teb200 {
 namespace kvc {
 
+// A sequence's queries within the packed rows and the tokens it holds; `bad`: the given numbers do not fit and were cut.
+struct SeqFit {
+  int q_row0, qlen, len;
+  bool bad;
+};
+
+__device__ __forceinline__ SeqFit fit_sequence(const int* cu_q, const int* kv_lens, int seq, int tq, int max_q, int max_kv) {
+  SeqFit f;
+  f.q_row0 = cu_q[seq];
+  f.qlen = cu_q[seq + 1] - f.q_row0;
+  f.len = kv_lens[seq];
+  f.bad = f.q_row0 < 0 || f.q_row0 > tq || f.qlen < 0 || f.qlen > max_q || f.qlen > tq - f.q_row0 || f.len < 0 || f.len > max_kv;
+  if (f.bad) {
+    f.q_row0 = min(max(f.q_row0, 0), tq);
+    f.qlen = min(min(max(f.qlen, 0), max_q), tq - f.q_row0);
+    f.len = min(max(f.len, 0), max_kv);
+  }
+  return f;
+}
+
 // The smallest power of two s with top <= 448 s, kept within 2^-60 .. 2^60.  With top = f 2^e, 1 <= f < 2, and
 // 448 = 1.75 2^8, that is 2^(e - 8) for f <= 1.75 and 2^(e - 7) above.
 __device__ __forceinline__ float scale_for(float top) {

@@ -200,19 +200,32 @@ __device__ __forceinline__ void expansion_extras(const Fp8GatherArgs& a) {
     out[i] = 0u;
   if (cta != 0 || threadIdx.x >= 32) return;
   const int lane = threadIdx.x;
-  int base = 0;
-  if (lane == 0) a.cu_k[0] = 0;
+  int base = 0, base_q = 0;
+  if (lane == 0) a.cu_k[0] = a.cut_q[0] = 0;
   for (int i0 = 0; i0 <= a.c.n; i0 += 32) {
     const int i = i0 + lane;
-    int x = i < a.c.n ? max(a.c.kv_lens[i], 0) : 0;
+    SeqFit f = {0, 0, 0, false};
+    if (i < a.c.n) f = fit_sequence(a.cu_q, a.c.kv_lens, i, a.tq, a.max_q, a.max_kv);
+    if (f.bad) atomicCAS(a.c.status, 0, kKvStatusPages);
+    int x = i < a.c.n ? max(a.c.kv_lens[i], 0) : 0, q = f.qlen;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      const int y = __shfl_up_sync(0xffffffffu, x, o), z = __shfl_up_sync(0xffffffffu, q, o);
+      if (lane >= o) {
+        x += y;
+        q += z;
+      }
     }
-    if (i < a.c.n) a.cu_k[i + 1] = base + x;
-    if (i <= a.c.n) a.first_row[i] = i * a.pitch;
+    if (i < a.c.n) {
+      a.cu_k[i + 1] = base + x;
+      a.cut_q[i + 1] = base_q + q;
+    }
+    if (i <= a.c.n) {
+      a.first_row[i] = i * a.pitch;
+      a.first_q[i] = f.q_row0;
+    }
     base += __shfl_sync(0xffffffffu, x, 31);
+    base_q += __shfl_sync(0xffffffffu, q, 31);
   }
 }
 
@@ -240,7 +253,7 @@ __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
   }
   int unseen_from = 0, unseen_to = 0;   // rows that nobody looks at
   if (a.off == nullptr && a.window_left >= 0) {
-    const int first_q = len - (a.cu_q[seq + 1] - a.cu_q[seq]);
+    const int first_q = len - fit_sequence(a.cu_q, a.c.kv_lens, seq, a.tq, a.max_q, a.max_kv).qlen;
     unseen_to = max(first_q - a.window_left, 0) / 128 * 128;
     unseen_from = min(a.sinks, 0x7fffff00) / 128 * 128 + (a.sinks % 128 != 0 ? 128 : 0);
   }
@@ -402,8 +415,8 @@ cudaError_t fp8_cache_append(const Fp8AppendArgs& a, cudaStream_t s) {
 cudaError_t fp8_cache_gather(const Fp8GatherArgs& a, cudaStream_t s) {
   if (!view_ok(a.c)) return cudaErrorInvalidValue;
   if (a.c.n == 0 || (a.rows == 0 && a.off != nullptr)) return cudaSuccess;
-  if (a.off == nullptr && (a.cu_q == nullptr || a.cu_k == nullptr || a.first_row == nullptr || a.out == nullptr || a.row_bytes % 4 != 0 ||
-                           static_cast<long long>(a.pitch) * a.c.n > a.rows))
+  if (a.off == nullptr && (a.cu_q == nullptr || a.cu_k == nullptr || a.first_row == nullptr || a.cut_q == nullptr || a.first_q == nullptr ||
+                           a.out == nullptr || a.row_bytes % 4 != 0 || static_cast<long long>(a.pitch) * a.c.n > a.rows))
     return cudaErrorInvalidValue;
   int blocks = (a.max_kv + 127) / 128 * 8;
   blocks = blocks < 1 ? 1 : (blocks > 65535 ? 65535 : blocks);

@@ -130,15 +130,16 @@ void fp8_cache_gather(const at::Tensor& k, const at::Tensor& v, const at::Tensor
   TORCH_CHECK(e == cudaSuccess, "fp8_cache_gather failed: ", cudaGetErrorString(e));
 }
 
-// Keys and values expanded for the packed attention kernel, pitch rows apart: {k, v, out, cumulative lengths, first rows};
-// out has its rows behind the last query zeroed and waits for the others.
+// Keys and values expanded for the packed attention kernel, pitch rows apart: {k, v, out, cumulative lengths and first rows
+// of the keys, those of the queries}; out has its rows behind the last query zeroed and waits for the others.
 std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
                                          const at::Tensor& vs, const at::Tensor& table, const at::Tensor& cu_q,
-                                         const at::Tensor& kv_lens, int64_t max_kv, int64_t window_left, int64_t sinks) {
+                                         const at::Tensor& kv_lens, int64_t max_q, int64_t max_kv, int64_t window_left, int64_t sinks) {
   c10::cuda::CUDAGuard guard(k.device());
   teb200::Fp8GatherArgs a;
   a.c = cache_view(k, v, ks, vs, table, kv_lens);
-  TORCH_CHECK(q.device() == k.device() && q.dim() == 3 && q.size(0) <= INT_MAX && sinks >= 0 && max_kv > 0 && max_kv <= INT_MAX - 128,
+  TORCH_CHECK(q.device() == k.device() && q.dim() == 3 && q.size(0) <= INT_MAX && sinks >= 0 && max_kv > 0 && max_kv <= INT_MAX - 128 && max_q >= 0 &&
+                  max_q <= INT_MAX,
               "attend: a size is out of range, or the queries are on another device than the cache");
   TORCH_CHECK(q.size(2) == a.c.d && q.size(1) % a.c.heads == 0 && q.size(1) > 0, "queries must be [tokens, heads, ", str(a.c.d),
               "] with a multiple of the cache's ", str(a.c.heads), " heads");
@@ -147,7 +148,7 @@ std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& 
   const at::Tensor ek = at::empty({pitch * a.c.n, a.c.heads, a.c.d}, q.options());
   const at::Tensor ev = at::empty_like(ek);
   const at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-  const at::Tensor meta = at::empty({2, a.c.n + 1}, cu_q.options());
+  const at::Tensor meta = at::empty({4, a.c.n + 1}, cu_q.options());
   a.dtype = value_type(q, "queries");
   a.out_k = ek.data_ptr();
   a.out_v = ev.data_ptr();
@@ -159,12 +160,15 @@ std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& 
   a.sinks = static_cast<int>(std::min(sinks, max_kv));
   a.cu_k = meta.data_ptr<int>();
   a.first_row = a.cu_k + a.c.n + 1;
+  a.cut_q = a.first_row + a.c.n + 1;
+  a.first_q = a.cut_q + a.c.n + 1;
+  a.max_q = static_cast<int>(max_q);
   a.out = out.data_ptr();
   a.tq = static_cast<int>(q.size(0));
   a.row_bytes = q.size(1) * q.size(2) * q.element_size();
   const cudaError_t e = teb200::fp8_cache_gather(a, cur_stream());
   TORCH_CHECK(e == cudaSuccess, "fp8_cache_expand failed: ", cudaGetErrorString(e));
-  return {ek, ev, out, meta.select(0, 0), meta.select(0, 1)};
+  return {ek, ev, out, meta.select(0, 0), meta.select(0, 1), meta.select(0, 2), meta.select(0, 3)};
 }
 
 at::Tensor fp8_cache_attend(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,

@@ -47,12 +47,16 @@ struct Fp8GatherArgs {
   int dtype = 0;
   // Expansion for the packed attention kernel: sequence i starts at row i * pitch and is followed by zeros up to the next
   // multiple of 128 rows; 128-row blocks that no query of the step sees are left out.  The launch also writes what that
-  // kernel needs beside it: cumulative lengths, first rows, and zeros in the output rows behind the last query.
+  // kernel needs beside it: cumulative lengths and first rows of keys and queries, cut to what the buffers hold (that
+  // kernel does not check them), and zeros in the output rows behind the last query.
   int pitch = 0;
   const int* cu_q = nullptr;    // [n + 1]
+  int max_q = 0;
   int window_left = -1, sinks = 0;
   int* cu_k = nullptr;          // [n + 1]
   int* first_row = nullptr;     // [n + 1]
+  int* cut_q = nullptr;         // [n + 1] cumulative queries
+  int* first_q = nullptr;       // [n + 1]
   void* out = nullptr;          // [tq, row_bytes]
   int tq = 0;
   long long row_bytes = 0;      // multiple of 4
