@@ -62,3 +62,17 @@ def test_offsets_out_of_order_stay_within_the_output(cu, expand, monkeypatch):
     cache, table = _filled(lens, 2, 64, 128, torch.Generator().manual_seed(2))
     o = kc.attend(_queries(70), cache, table, _i32(cu), _i32(lens), max_q=70, max_kv=300)
     assert _reported() and o.shape == (70, 8, 128)
+
+
+@both_paths
+def test_sequences_longer_than_max_kv_are_cut_and_reported(expand, monkeypatch):
+    _path(monkeypatch, expand)
+    lens = [300, 90, 260]
+    cache, table = _filled(lens, 2, 64, 128, torch.Generator().manual_seed(3))
+    q, cu = _queries(130), _i32([0, 80, 90, 130])
+    want = kc.attend(q, cache, table, cu, _i32([200, 90, 200]), max_q=80, max_kv=200)
+    assert not _reported()
+    got = kc.attend(q, cache, table, cu, _i32(lens), max_q=80, max_kv=200)
+    assert _reported() and torch.equal(got, want)
+    got = kc.attend(q, cache, table, cu, _i32([200, -90, 200]), max_q=80, max_kv=200)
+    assert _reported() and (got[80:90] == 0).all() and torch.equal(got[:80], want[:80])

@@ -207,7 +207,7 @@ __device__ __forceinline__ void expansion_extras(const Fp8GatherArgs& a) {
     SeqFit f = {0, 0, 0, false};
     if (i < a.c.n) f = fit_sequence(a.cu_q, a.c.kv_lens, i, a.tq, a.max_q, a.max_kv);
     if (f.bad) atomicCAS(a.c.status, 0, kKvStatusPages);
-    int x = i < a.c.n ? max(a.c.kv_lens[i], 0) : 0, q = f.qlen;
+    int x = f.len, q = f.qlen;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o), z = __shfl_up_sync(0xffffffffu, q, o);
@@ -244,16 +244,22 @@ __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
   const int head = is_v ? unit - a.c.heads : unit;
   const int seq = blockIdx.z;
   const int per = a.c.page_size / kKvBlock;
-  const int len = a.c.kv_lens[seq];
+  int len, first_q = 0;
+  if (a.off != nullptr) {
+    len = a.c.kv_lens[seq];
+  } else {
+    const SeqFit f = fit_sequence(a.cu_q, a.c.kv_lens, seq, a.tq, a.max_q, a.max_kv);
+    len = f.len;                // a longer sequence is cut, as where the codes are read in place
+    first_q = f.len - f.qlen;
+  }
   const int off = a.off != nullptr ? a.off[seq] : seq * a.pitch;
   const int stop = a.off == nullptr ? (len + 127) / 128 * 128 : len;
-  if (len < 0 || off < 0 || stop > (a.off == nullptr ? a.pitch : a.rows - off)) {
+  if (len < 0 || off < 0 || stop > (a.off == nullptr ? a.pitch : a.rows - off)) {   // (never in an expansion)
     if (lane == 0) atomicCAS(a.c.status, 0, kKvStatusPages);
     return;
   }
   int unseen_from = 0, unseen_to = 0;   // rows that nobody looks at
   if (a.off == nullptr && a.window_left >= 0) {
-    const int first_q = len - fit_sequence(a.cu_q, a.c.kv_lens, seq, a.tq, a.max_q, a.max_kv).qlen;
     unseen_to = max(first_q - a.window_left, 0) / 128 * 128;
     unseen_from = min(a.sinks, 0x7fffff00) / 128 * 128 + (a.sinks % 128 != 0 ? 128 : 0);
   }

@@ -43,7 +43,7 @@ struct Fp8GatherArgs {
   void* out_v = nullptr;
   const int* off = nullptr;     // [n] first row of every sequence (nullptr: expansion, below)
   int rows = 0;
-  int max_kv = 0;               // longest sequence (sizes the grid, longer ones are handled)
+  int max_kv = 0;               // longest sequence (sizes the grid, longer ones are handled; an expansion cuts them there)
   int dtype = 0;
   // Expansion for the packed attention kernel: sequence i starts at row i * pitch and is followed by zeros up to the next
   // multiple of 128 rows; 128-row blocks that no query of the step sees are left out.  The launch also writes what that
