@@ -76,3 +76,18 @@ def test_sequences_longer_than_max_kv_are_cut_and_reported(expand, monkeypatch):
     assert _reported() and torch.equal(got, want)
     got = kc.attend(q, cache, table, cu, _i32([200, -90, 200]), max_q=80, max_kv=200)
     assert _reported() and (got[80:90] == 0).all() and torch.equal(got[:80], want[:80])
+
+
+@both_paths
+def test_queries_beyond_max_q_are_zero_and_reported(expand, monkeypatch):
+    _path(monkeypatch, expand)
+    lens = [300, 90, 260]
+    cache, table = _filled(lens, 2, 64, 128, torch.Generator().manual_seed(4))
+    q, cu = _queries(141), _cum([100, 10, 30])
+    keep = list(range(64)) + list(range(100, 140))
+    want = kc.attend(q[keep], cache, table, _i32(_cum([64, 10, 30])), _i32(lens), max_q=64, max_kv=300)
+    assert not _reported()
+    _litter(q)
+    got = kc.attend(q, cache, table, _i32(cu), _i32(lens), max_q=64, max_kv=300)
+    assert _reported() and torch.equal(got[keep], want)
+    assert (got[64:100] == 0).all() and (got[140:] == 0).all()

@@ -184,8 +184,8 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
     Sequence i's queries are rows ``cu_q[i] .. cu_q[i + 1]`` (``cu_q[0]`` is 0) and, under the causal mask, the LAST tokens of its
     ``kv_lens[i]`` (bottom-right alignment).  ``window = (left, right)`` limits what the query at position p sees to keys
     ``p - left .. p``, plus the first ``sink_tokens`` tokens; -1 leaves a side open, and the right side is the causal
-    one.  ``max_q`` / ``max_kv`` bound the queries and tokens of a sequence.  Rows that see nothing, and rows behind the
-    last sequence, are zero.  There is no backward pass."""
+    one.  ``max_q`` / ``max_kv`` bound the queries and tokens of a sequence: a longer one is cut there and reported.  Rows
+    that see nothing, rows behind the last sequence, and rows that were cut off are zero.  There is no backward pass."""
     if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("attention over the 8-bit cache has no backward pass: call it under torch.no_grad()")
     left = -1

@@ -595,16 +595,8 @@ __global__ void __launch_bounds__(kWarps * 32, (Tune<D, NT>::kCtas)) attend_kern
   __shared__ int sm_scan[kWarps], sm_at[2], sm_total;
   const Fp8AttendArgs& a = p.a;
   cudaTriggerProgrammaticLaunchCompletion();   // the joining kernel may be launched (it waits for this one's end)
-  {
-    // queries behind the last sequence: zeros
-    const long long first = static_cast<long long>(max(a.cu_q[a.c.n], 0)) * a.hq * (D / 2);
-    const long long last = static_cast<long long>(a.tq) * a.hq * (D / 2);
-    const long long cta = static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x;
-    uint32_t* o = reinterpret_cast<uint32_t*>(a.out);
-    for (long long i = first + cta * blockDim.x + threadIdx.x; i < last;
-         i += static_cast<long long>(gridDim.x) * gridDim.y * blockDim.x)
-      o[i] = 0u;
-  }
+  zero_unclaimed(reinterpret_cast<uint32_t*>(a.out), static_cast<long long>(a.hq) * (D / 2), a.cu_q, a.c.n, a.tq, a.max_q,
+                 static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x, static_cast<long long>(gridDim.x) * gridDim.y);
   if (a.c.n == 0) return;
   Run run;
   if (p.ctas == 0) {

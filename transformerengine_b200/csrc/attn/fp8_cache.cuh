@@ -29,6 +29,25 @@ __device__ __forceinline__ SeqFit fit_sequence(const int* cu_q, const int* kv_le
   return f;
 }
 
+// Zeros in the output rows (of `words` 32-bit words) that no query claims: behind the last sequence, and, reported by
+// fit_sequence, those of a sequence beyond max_q.  All threads of `ctas` CTAs take part.
+__device__ __forceinline__ void zero_unclaimed(uint32_t* out, long long words, const int* cu_q, int n, int tq, int max_q,
+                                               long long cta, long long ctas) {
+  const int end = cu_q[n];
+  int q0 = cta < n ? cu_q[cta] : 0, q1 = cta < n ? cu_q[cta + 1] : 0;   // the first (mostly the only) turn of the loop below
+  for (long long i = max(end, 0) * words + cta * blockDim.x + threadIdx.x; i < tq * words; i += ctas * blockDim.x) out[i] = 0u;
+  for (long long seq = cta; seq < n;) {
+    const int from = min(max(q0, 0), tq);
+    const int claimed = min(min(max(q1 - q0, 0), max_q), tq - from);
+    for (long long i = (from + claimed) * words + threadIdx.x; i < min(q1, tq) * words; i += blockDim.x) out[i] = 0u;
+    seq += ctas;
+    if (seq < n) {
+      q0 = cu_q[seq];
+      q1 = cu_q[seq + 1];
+    }
+  }
+}
+
 // The smallest power of two s with top <= 448 s, kept within 2^-60 .. 2^60.  With top = f 2^e, 1 <= f < 2, and
 // 448 = 1.75 2^8, that is 2^(e - 8) for f <= 1.75 and 2^(e - 7) above.
 __device__ __forceinline__ float scale_for(float top) {

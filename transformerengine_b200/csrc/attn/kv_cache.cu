@@ -190,14 +190,11 @@ __device__ __forceinline__ void store8<__half>(__half* p, const float (&y)[8]) {
                                             pack2<false>(y[4], y[5]), pack2<false>(y[6], y[7]));
 }
 
-// What the packed attention kernel needs beside the expanded keys and values (CTA 0), and zeros behind the last query.
+// What the packed attention kernel needs beside the expanded keys and values (CTA 0), and zeros in the rows without a query.
 __device__ __forceinline__ void expansion_extras(const Fp8GatherArgs& a) {
   const long long cta = (static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
   const long long ctas = static_cast<long long>(gridDim.x) * gridDim.y * gridDim.z;
-  const long long words = a.row_bytes / 4;
-  uint32_t* out = static_cast<uint32_t*>(a.out);
-  for (long long i = max(a.cu_q[a.c.n], 0) * words + cta * blockDim.x + threadIdx.x; i < a.tq * words; i += ctas * blockDim.x)
-    out[i] = 0u;
+  zero_unclaimed(static_cast<uint32_t*>(a.out), a.row_bytes / 4, a.cu_q, a.c.n, a.tq, a.max_q, cta, ctas);
   if (cta != 0 || threadIdx.x >= 32) return;
   const int lane = threadIdx.x;
   int base = 0, base_q = 0;

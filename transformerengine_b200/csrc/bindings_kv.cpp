@@ -131,7 +131,7 @@ void fp8_cache_gather(const at::Tensor& k, const at::Tensor& v, const at::Tensor
 }
 
 // Keys and values expanded for the packed attention kernel, pitch rows apart: {k, v, out, cumulative lengths and first rows
-// of the keys, those of the queries}; out has its rows behind the last query zeroed and waits for the others.
+// of the keys, those of the queries}; out has the rows that no query claims zeroed and waits for the others.
 std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
                                          const at::Tensor& vs, const at::Tensor& table, const at::Tensor& cu_q,
                                          const at::Tensor& kv_lens, int64_t max_q, int64_t max_kv, int64_t window_left, int64_t sinks) {

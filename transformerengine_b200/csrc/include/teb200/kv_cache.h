@@ -48,7 +48,7 @@ struct Fp8GatherArgs {
   // Expansion for the packed attention kernel: sequence i starts at row i * pitch and is followed by zeros up to the next
   // multiple of 128 rows; 128-row blocks that no query of the step sees are left out.  The launch also writes what that
   // kernel needs beside it: cumulative lengths and first rows of keys and queries, cut to what the buffers hold (that
-  // kernel does not check them), and zeros in the output rows behind the last query.
+  // kernel does not check them), and zeros in the output rows that no query claims.
   int pitch = 0;
   const int* cu_q = nullptr;    // [n + 1]
   int max_q = 0;
