@@ -91,3 +91,49 @@ def test_queries_beyond_max_q_are_zero_and_reported(expand, monkeypatch):
     got = kc.attend(q, cache, table, _i32(cu), _i32(lens), max_q=64, max_kv=300)
     assert _reported() and torch.equal(got[keep], want)
     assert (got[64:100] == 0).all() and (got[140:] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------- pages not held
+@both_paths
+@pytest.mark.parametrize("bad", [-1, 10 ** 6])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_pages_that_are_not_held_read_as_zeros_and_are_reported(bad, d, expand, monkeypatch):
+    if expand and d != 128:
+        pytest.skip("the expansion serves head dim 128")
+    _path(monkeypatch, expand)
+    lens, qs = [300, 200, 130], [70, 1, 5]
+    cache, table = _filled(lens, 2, 64, d, torch.Generator().manual_seed(5))
+    cache = kc.FP8KVCache(*(torch.cat([t.view(torch.uint8), torch.zeros_like(t.view(torch.uint8)[:1])]).view(t.dtype) for t in cache))
+    cache.k_scale[-1], cache.v_scale[-1] = 1.0, 1.0
+    zeros = table.clone()
+    table[0, 1], table[1, 3], zeros[0, 1], zeros[1, 3] = bad, bad, len(cache.k) - 1, len(cache.k) - 1
+    q, kw = _queries(sum(qs), d=d), dict(max_q=70, max_kv=300)
+    want = kc.attend(q, cache, zeros, _i32(_cum(qs)), _i32(lens), **kw)
+    assert not _reported()
+    got = kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), **kw)
+    assert _reported() and torch.equal(got, want)
+    # and on the CPU (fp32; the kernels round the probabilities to the type or to fp16, the result to the type)
+    ref = kc.attend(q.cpu(), kc.FP8KVCache(*(t.cpu() for t in cache)), table.clamp(max=len(cache.k)).masked_fill(table == bad, -1).cpu(),
+                    _i32(_cum(qs)).cpu(), _i32(lens).cpu(), **kw)
+    assert ((got.cpu().float() - ref.float()).abs() <= 2 * 2.0 ** -8 * ref.abs().float() + 2 * 2.0 ** -8 * 6.0).all()
+    # a table that ends before the sequence does
+    got = kc.attend(q, cache, zeros[:, :3].contiguous(), _i32(_cum(qs)), _i32(lens), **kw)
+    zeros[0, 3:] = len(cache.k) - 1
+    assert _reported() and torch.equal(got[:70], kc.attend(q, cache, zeros, _i32(_cum(qs)), _i32(lens), **kw)[:70])
+
+
+@both_paths
+def test_pages_out_of_sight_are_not_reported(expand, monkeypatch):
+    _path(monkeypatch, expand)
+    lens, qs = [300, 200, 500], [20, 0, 33]
+    cache, table = _filled(lens, 2, 32, 128, torch.Generator().manual_seed(6))
+    q, kw = _queries(53), dict(max_q=33, max_kv=500, window=(40, 0), sink_tokens=20)
+    want = kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), **kw)
+    table[1] = -1                                       # nobody asks
+    table[0, 1:(300 - 20 - 40) // 32] = -1              # between the sinks and the first query's window
+    table[2, 1:(500 - 33 - 40) // 32] = -1
+    got = kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), **kw)
+    assert not _reported() and torch.equal(got, want)
+    table[2, (500 - 33 - 40) // 32] = -1                # its last tokens are within the window
+    kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), **kw)
+    assert _reported()

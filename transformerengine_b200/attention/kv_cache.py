@@ -10,7 +10,8 @@ On CUDA every function runs the kernels of ``csrc/attn/kv_cache.cu`` and ``csrc/
 stream (head dims 64, 128, 256); the PyTorch bodies below are the CPU path and the oracle of the kernel tests (any head
 dim).  Sequence i owns row i of ``page_table`` (int32 ``[n, width]``, the page of every ``page_size`` tokens, -1 where
 none is held) and ``kv_lens[i]`` tokens.  Ids outside the cache and lengths that do not fit are skipped by the kernels and
-reported by :func:`transformerengine_b200.check_status`; no function synchronizes with the device.
+reported by :func:`transformerengine_b200.check_status`; attention takes the keys and values of a page that is not held for
+zeros, and reports it where a query sees it.  No function synchronizes with the device.
 """
 from __future__ import annotations
 

@@ -242,14 +242,14 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
           look_k = a.c.k_scale[look_idx];
           look_v = a.c.v_scale[look_idx];
         } else {
-          // a page that is not held may lie outside what the tile sees; inside, its tokens count as hidden
+          // a page that is not held may lie outside what the tile sees; inside, it is reported and its tokens are zeros
           if (tok <= hi_max && (tok + kKvBlock > lo_min || tok < a.sinks)) atomicCAS(a.c.status, 0, kKvStatusPages);
         }
       }
     }
   };
-  // start the copies of the keys (values) of the warp's n-th step; blocks that are not held: block 0, whose tokens are then
-  // hidden.  One group each, in the order k0 v0 k1 v1 ...
+  // start the copies of the keys (values) of the warp's n-th step; blocks that are not held: block 0, whose codes nobody
+  // uses.  One group each, in the order k0 v0 k1 v1 ...
   auto fetch = [&](int n, bool values) {
     const int st = s_begin + warp + n * kWarps;
     if (st < s_end) {
@@ -409,6 +409,14 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[t][b][e] = fmaf(s[t][b][e], c[e & 1], lv);
       }
+    if (!all_held) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        if (!held[b]) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s[t][b][0] = s[t][b][1] = s[t][b][2] = s[t][b][3] = 0.f;   // zero keys (V scale: 1)
+        }
+    }
     if (need_mask) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -417,7 +425,7 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int tok = tok0 + b * kKvBlock + g8 + (e >> 1) * 8;
-            const bool seen = held[b] && tok <= hi[t][e & 1] && (tok >= lo[t][e & 1] || tok < a.sinks);
+            const bool seen = tok <= hi[t][e & 1] && (tok >= lo[t][e & 1] || tok < a.sinks);
             if (!seen) s[t][b][e] = -INFINITY;
           }
     }
@@ -466,7 +474,8 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
     cp_async_wait<2 * kStages - 1>();
     __syncwarp();
     if (need_mask) {
-      // tokens hidden from all rows meet probability 0, but what their slots hold may be NaN: zeros in their place
+      // tokens hidden from all rows meet probability 0, but what their slots hold may be NaN: zeros in their place, and in
+      // that of tokens whose page is not held
       const uint32_t stage = ring + n % kStages * kStageBytes + kStepBytes;
       for (int x = lane; x < STEP * (D / 16); x += 32) {
         const int row = x / (D / 16), tok = tok0 + row;

@@ -227,7 +227,8 @@ __device__ __forceinline__ void expansion_extras(const Fp8GatherArgs& a) {
 }
 
 // One warp per (sequence, 16-token block, K or V, head): codes * scale into a token-major buffer.  Blocks whose page is
-// not held, and the rows from a sequence's end to the next multiple of 128 (expansion), become zeros.
+// not held, and the rows from a sequence's end to the next multiple of 128 (expansion), become zeros.  An expansion reports
+// pages that are not held where a query sees them, as attention in place does.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
   constexpr int kLanesPerRow = D / 8;
@@ -248,6 +249,7 @@ __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
     const SeqFit f = fit_sequence(a.cu_q, a.c.kv_lens, seq, a.tq, a.max_q, a.max_kv);
     len = f.len;                // a longer sequence is cut, as where the codes are read in place
     first_q = f.len - f.qlen;
+    if (f.qlen == 0) len = 0;   // nobody looks
   }
   const int off = a.off != nullptr ? a.off[seq] : seq * a.pitch;
   const int stop = a.off == nullptr ? (len + 127) / 128 * 128 : len;
@@ -256,8 +258,10 @@ __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
     return;
   }
   int unseen_from = 0, unseen_to = 0;   // rows that nobody looks at
+  int seen_from = 0;                    // first row in a window
   if (a.off == nullptr && a.window_left >= 0) {
-    unseen_to = max(first_q - a.window_left, 0) / 128 * 128;
+    seen_from = max(first_q - a.window_left, 0);
+    unseen_to = seen_from / 128 * 128;
     unseen_from = min(a.sinks, 0x7fffff00) / 128 * 128 + (a.sinks % 128 != 0 ? 128 : 0);
   }
   T* out = static_cast<T*>(is_v ? a.out_v : a.out_k) + static_cast<long long>(off) * a.c.heads * D + head * D +
@@ -268,10 +272,11 @@ __global__ void __launch_bounds__(128) gather_kernel(const Fp8GatherArgs a) {
     int page = -1;
     if (blk * kKvBlock < len) {
       page = slot < a.c.width ? a.c.table[static_cast<long long>(seq) * a.c.width + slot] : a.c.pages;
-      if (page >= a.c.pages) {
+      const bool wanted = blk * kKvBlock + kKvBlock > seen_from || blk * kKvBlock < a.sinks;   // by the step's queries
+      if (a.off != nullptr ? page >= a.c.pages : wanted && (page < 0 || page >= a.c.pages)) {
         if (lane == 0) atomicCAS(a.c.status, 0, kKvStatusPages);
-        page = -1;
       }
+      if (page >= a.c.pages) page = -1;
     }
     const long long idx = page < 0 ? 0 : (static_cast<long long>(page) * a.c.heads + head) * per + blk % per;
     const uint8_t* codes = (is_v ? a.c.v : a.c.k) + idx * (kKvBlock * D) + lane * 8;
