@@ -137,3 +137,21 @@ def test_pages_out_of_sight_are_not_reported(expand, monkeypatch):
     table[2, (500 - 33 - 40) // 32] = -1                # its last tokens are within the window
     kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), **kw)
     assert _reported()
+
+
+# ----------------------------------------------------------------------------------------------- layouts and sizes
+def test_a_cache_at_an_odd_address_is_refused():
+    pool = torch.zeros(2 * 2 * 16 * 64 + 8, dtype=torch.uint8, device="cuda")
+    odd = pool[8:].view(2, 2, 16, 64).view(torch.float8_e4m3fn)
+    cache = kc.FP8KVCache.allocate(2, 2, 16, 64, device="cuda")
+    x = torch.zeros(1, 2, 64, device="cuda", dtype=torch.bfloat16)
+    one = (_i32([[0]]), _i32([0, 1]), _i32([1]))
+    for bad in (cache._replace(k=odd), cache._replace(v=odd)):
+        with pytest.raises(RuntimeError, match="16 bytes"):
+            kc.append(bad, x, x, *one)
+        with pytest.raises(RuntimeError, match="16 bytes"):
+            kc.attend(x, bad, *one, max_q=1, max_kv=1)
+        with pytest.raises(RuntimeError, match="16 bytes"):
+            kc.gather(bad, one[0], one[2], _i32([0]), 1, torch.bfloat16)
+        kc.copy_pages([bad], [0], [1])                 # copies take any address
+    te.check_status()

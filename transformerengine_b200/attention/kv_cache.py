@@ -30,7 +30,7 @@ _MAX_EXP = 60
 
 class FP8KVCache(NamedTuple):
     """The 8-bit cache of one layer (:meth:`allocate` makes an empty one, :func:`append` fills it: scales that are not
-    powers of two give wrong results)."""
+    powers of two give wrong results).  On CUDA the codes start on a multiple of 16 bytes."""
 
     k: torch.Tensor          # float8_e4m3fn [pages, heads, page_size, d]
     v: torch.Tensor

@@ -44,6 +44,9 @@ teb200::Fp8CacheView cache_view(const at::Tensor& k, const at::Tensor& v, const 
               "the cache must be contiguous [pages, heads, page_size, d] codes, k and v alike");
   TORCH_CHECK(k.scalar_type() == at::kFloat8_e4m3fn && v.scalar_type() == at::kFloat8_e4m3fn,
               "the cache's codes must be float8_e4m3fn");
+  // (a contiguous view into a pool may start anywhere; the kernels copy 16 bytes at a time)
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(k.data_ptr()) | reinterpret_cast<uintptr_t>(v.data_ptr())) % 16 == 0,
+              "the cache's codes must start on a multiple of 16 bytes");
   const int64_t page = k.size(2), d = k.size(3);
   TORCH_CHECK(d == 64 || d == 128 || d == 256, "the 8-bit cache kernels take head dims 64, 128 and 256, got ", str(d));
   TORCH_CHECK(page >= teb200::kKvBlock && page % teb200::kKvBlock == 0, "the page size must be a multiple of ",
