@@ -155,3 +155,27 @@ def test_a_cache_at_an_odd_address_is_refused():
             kc.gather(bad, one[0], one[2], _i32([0]), 1, torch.bfloat16)
         kc.copy_pages([bad], [0], [1])                 # copies take any address
     te.check_status()
+
+
+@both_paths
+@pytest.mark.parametrize("qs", [[1, 1, 1], [3, 0, 40]])
+def test_max_q_may_be_any_bound(qs, expand, monkeypatch):
+    _path(monkeypatch, expand)
+    lens = [300, 0, 5000]
+    cache, table = _filled(lens, 2, 64, 128, torch.Generator().manual_seed(7))
+    q = _queries(sum(qs))
+    want = kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_q=sum(qs), max_kv=5000)
+    for loose in (10 ** 6, 2 ** 31 - 1, 2 ** 40):
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        assert torch.equal(want, kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_q=loose, max_kv=5000))
+        assert torch.cuda.max_memory_allocated() - held < 2 ** 27
+    te.check_status()
+
+
+def test_no_query_rows_with_a_large_max_q():
+    cache, table = _filled([300] * 4, 8, 64, 128, torch.Generator().manual_seed(8))
+    q = torch.zeros(0, 64, 128, device="cuda", dtype=torch.bfloat16)
+    o = kc.attend(q, cache, table, _i32([0] * 5), _i32([300] * 4), max_q=500, max_kv=300)
+    assert o.shape == (0, 64, 128)
+    te.check_status()

@@ -203,8 +203,9 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
         scale = d ** -0.5
     if not _cuda(cache):
         return _attend_ref(q, cache, page_table, cu_q, kv_lens, scale, causal, left, sink_tokens)
+    max_q = min(max_q, q.shape[0])     # it sizes launches and buffers: no sequence has more
     # (the packed kernels take the maximum of the raw scores: a positive scale)
-    if d == 128 and scale > 0.0 and max_kv > 0 and _expands(page_table.shape[0], hq, cache.k.shape[1], max_q):
+    if d == 128 and scale > 0.0 and max_q > 0 and max_kv > 0 and _expands(page_table.shape[0], hq, cache.k.shape[1], max_q):
         return _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
     return _ext.get().fp8_cache_attend(q, *cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
 

@@ -813,7 +813,9 @@ cudaError_t launch(AttendParams p, cudaStream_t s) {
     ready.fetch_or(uint64_t{1} << (dev & 63), std::memory_order_relaxed);
   }
   if (p.ctas == 0) {
-    const dim3 grid(p.a.c.heads * p.row_tiles, p.a.c.n > 0 ? p.a.c.n : 1);
+    const long long width = static_cast<long long>(p.a.c.heads) * p.row_tiles;
+    if (width > 0x7fffffff) return cudaErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(width), p.a.c.n > 0 ? p.a.c.n : 1);
     attend_kernel<D, NT, BF><<<grid, kWarps * 32, kSmem, s>>>(p);
     return cudaGetLastError();
   }

@@ -141,8 +141,7 @@ std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& 
   c10::cuda::CUDAGuard guard(k.device());
   teb200::Fp8GatherArgs a;
   a.c = cache_view(k, v, ks, vs, table, kv_lens);
-  TORCH_CHECK(q.device() == k.device() && q.dim() == 3 && q.size(0) <= INT_MAX && sinks >= 0 && max_kv > 0 && max_kv <= INT_MAX - 128 && max_q >= 0 &&
-                  max_q <= INT_MAX,
+  TORCH_CHECK(q.device() == k.device() && q.dim() == 3 && q.size(0) <= INT_MAX && sinks >= 0 && max_kv > 0 && max_kv <= INT_MAX - 128 && max_q >= 0,
               "attend: a size is out of range, or the queries are on another device than the cache");
   TORCH_CHECK(q.size(2) == a.c.d && q.size(1) % a.c.heads == 0 && q.size(1) > 0, "queries must be [tokens, heads, ", str(a.c.d),
               "] with a multiple of the cache's ", str(a.c.heads), " heads");
@@ -165,7 +164,7 @@ std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& 
   a.first_row = a.cu_k + a.c.n + 1;
   a.cut_q = a.first_row + a.c.n + 1;
   a.first_q = a.cut_q + a.c.n + 1;
-  a.max_q = static_cast<int>(max_q);
+  a.max_q = static_cast<int>(std::min(max_q, q.size(0)));
   a.out = out.data_ptr();
   a.tq = static_cast<int>(q.size(0));
   a.row_bytes = q.size(1) * q.size(2) * q.element_size();
@@ -183,8 +182,7 @@ at::Tensor fp8_cache_attend(const at::Tensor& q, const at::Tensor& k, const at::
   TORCH_CHECK(q.dim() == 3 && q.size(2) == a.c.d && q.size(1) % a.c.heads == 0 && q.size(1) > 0,
               "queries must be [tokens, heads, ", str(a.c.d), "] with a multiple of the cache's ", str(a.c.heads), " heads");
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "queries must be fp16 or bf16");
-  TORCH_CHECK(q.device() == k.device() && q.size(0) <= INT_MAX && max_q <= INT_MAX && max_kv <= INT_MAX && max_q >= 0 &&
-                  max_kv >= 0 && sinks >= 0,
+  TORCH_CHECK(q.device() == k.device() && q.size(0) <= INT_MAX && max_kv <= INT_MAX && max_q >= 0 && max_kv >= 0 && sinks >= 0,
               "attend: a size is out of range, or the queries are on another device than the cache");
   const at::Tensor qr = rows16(q);
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
@@ -195,7 +193,7 @@ at::Tensor fp8_cache_attend(const at::Tensor& q, const at::Tensor& k, const at::
   a.tq = static_cast<int>(q.size(0));
   a.hq = static_cast<int>(q.size(1));
   a.is_bf16 = q.scalar_type() == at::kBFloat16;
-  a.max_q = static_cast<int>(max_q);
+  a.max_q = static_cast<int>(std::min(max_q, q.size(0)));   // it sizes the launch: no sequence has more
   a.max_kv = static_cast<int>(max_kv);
   a.causal = causal;
   a.window_left = static_cast<int>(window_left < 0 ? -1 : std::min(window_left, max_kv));   // no key lies further back
