@@ -179,3 +179,57 @@ def test_no_query_rows_with_a_large_max_q():
     o = kc.attend(q, cache, table, _i32([0] * 5), _i32([300] * 4), max_q=500, max_kv=300)
     assert o.shape == (0, 64, 128)
     te.check_status()
+
+
+# --------------------------------------------------------------------------------------- which path, and its memory
+def _peak(call):
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    out = call()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - held
+
+
+def test_a_chunk_beside_decoding_sequences():
+    """One prompt chunk among single tokens: read in place, as 63 of the sequences would be."""
+    lens, qs = [900 + 13 * i for i in range(64)], [1] * 64
+    qs[17] = 300
+    cache, table = _filled(lens, 8, 64, 128, torch.Generator().manual_seed(9))
+    q = _queries(sum(qs), heads=32)
+    o, used = _peak(lambda: kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_q=300, max_kv=max(lens)))
+    assert used < 2 ** 26                               # the expansion would take 0.5 GB
+    each = [kc.attend(q[a:b], cache, table[i:i + 1], _i32([0, b - a]), _i32(lens[i:i + 1]), max_q=b - a, max_kv=lens[i])
+            for i, (a, b) in enumerate(zip(_cum(qs), _cum(qs)[1:]))]
+    # both round the probabilities (2^-11, or 2^-8 where the chunk alone is expanded) and the result once; |v| < 6
+    err = (o.float() - torch.cat(each).float()).abs()
+    assert (err <= 2.0 ** -7 * o.abs().float() + 2 * 2.0 ** -8 * 6.0).all()
+    te.check_status()
+
+
+@pytest.mark.parametrize("window", [-1, 500])
+def test_a_loose_max_kv_takes_bounded_memory(window):
+    lens, qs = [700, 300, 80], [300, 200, 80]
+    cache, table = _filled(lens, 8, 64, 128, torch.Generator().manual_seed(10))
+    q, kw = _queries(sum(qs), heads=32), dict(max_q=300, window=(window, 0), sink_tokens=4)
+    want = kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_kv=700, **kw)
+    for loose in (10 ** 6, 4 * 10 ** 6, 2 ** 31 - 1):
+        o, used = _peak(lambda: kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_kv=loose, **kw))
+        assert used <= kc._EXPAND_BYTES + 2 ** 26
+        # one path against the other: rounding of the probabilities to 8 and 11 bits, and of the result, |v| < 6
+        assert ((o.float() - want.float()).abs() <= 2.0 ** -7 * want.abs().float() + 2 * 2.0 ** -8 * 6.0).all()
+    te.check_status()
+
+
+def test_sequences_expanded_in_groups_give_the_same(monkeypatch):
+    _path(monkeypatch, True)
+    lens, qs = [700, 300, 80, 1000, 64], [100, 0, 80, 130, 3]
+    cache, table = _filled(lens, 2, 64, 128, torch.Generator().manual_seed(11))
+    q = _queries(sum(qs) + 7)
+    run = lambda: kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_q=130, max_kv=1000)  # noqa: E731
+    want = run()
+    for groups in (2, 3, 5):
+        monkeypatch.setattr(kc, "_EXPAND_BYTES", kc._expansion_bytes(8, 2, 128, 130, 1000) * -(-5 // groups))
+        _litter(q)
+        assert torch.equal(run(), want)
+    te.check_status()

@@ -163,18 +163,29 @@ def gather(cache: FP8KVCache, page_table: torch.Tensor, kv_lens: torch.Tensor, o
     return k, v
 
 
-def _expands(n: int, hq: int, hk: int, max_q: int) -> bool:
+_EXPAND_BYTES = 4 << 30      # of expanded keys and values at a time, 2 % of the device's memory; needs beyond are read in place
+
+
+def _expansion_bytes(hq: int, hk: int, d: int, max_q: int, max_kv: int) -> int:
+    """Buffers that one sequence takes where its codes are expanded: keys and values in 16 bits, row sums."""
+    return 4 * hk * d * (-(-max_kv // 128) * 128) + 4 * hq * (-(-max_q // 128) * 128)
+
+
+def _expands(n: int, hq: int, hk: int, d: int, max_q: int, tokens: int, max_kv: int) -> bool:
     """Whether expanding the codes once for the packed 16-bit attention kernel beats the kernel that reads them in place.
 
     The latter walks the cache once for every 16 query rows of a key head (4.3e-5 us per tile and token on all SMs), the
     former takes 0.02 us per token and wave of its CTAs (256 queries of a head each).  Measured, us in place / expanded,
     32 / 8 heads: 8 sequences of 8000 tokens, 32 queries 187 / 328, 64 queries 350 / 330, 128 queries 670 / 333; one of
-    100000, 128 queries 985 / 1597; 64 of 2000, 64 queries 790 / 649."""
+    100000, 128 queries 985 / 1597; 64 of 2000, 64 queries 790 / 649.  Both counts are bounded by the packed queries
+    (``tokens``) too: beside a prompt chunk the other sequences may have a token each (1024 queries beside 63 single ones on
+    500 - 8000 tokens: 1016 / 1485).  Sequences whose expansion would
+    not fit ``_EXPAND_BYTES`` one at a time (a ``max_kv`` far above the lengths, say) are read in place."""
     rows = hq // hk * max_q
-    if rows <= 64:
+    if rows <= 64 or _expansion_bytes(hq, hk, d, max_q, max_kv) > _EXPAND_BYTES:
         return False
-    waves = -(-n * hq * -(-max_q // 256) // 148)
-    return n * hk * -(-rows // 16) > 470 * waves
+    waves = -(-hq * min(n * -(-max_q // 256), tokens // 256 + n) // 148)
+    return hk * min(n * -(-rows // 16), hq // hk * tokens // 16 + n) > 470 * waves
 
 
 def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, *,
@@ -205,17 +216,27 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
         return _attend_ref(q, cache, page_table, cu_q, kv_lens, scale, causal, left, sink_tokens)
     max_q = min(max_q, q.shape[0])     # it sizes launches and buffers: no sequence has more
     # (the packed kernels take the maximum of the raw scores: a positive scale)
-    if d == 128 and scale > 0.0 and max_q > 0 and max_kv > 0 and _expands(page_table.shape[0], hq, cache.k.shape[1], max_q):
+    if d == 128 and scale > 0.0 and max_q > 0 and max_kv > 0 and _expands(page_table.shape[0], hq, cache.k.shape[1], d, max_q,
+                                                                                q.shape[0], max_kv):
         return _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
     return _ext.get().fp8_cache_attend(q, *cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens)
 
 
 def _attend_expanded(q, cache, page_table, cu_q, kv_lens, max_q, max_kv, scale, causal, left, sink_tokens):
     """Codes expanded to 16 bits (every sequence padded to whole 128-token blocks with zeros), then the packed attention
-    kernel: prompt chunks are bound by its products, not by the cache."""
-    k, v, out, cu_k, first_k, cut_q, first_q = _ext.get().fp8_cache_expand(q, *cache, page_table, cu_q, kv_lens, max_q, max_kv, left,
-                                                                           sink_tokens)
-    return _flash.flash_varlen_forward(q, k, v, out, cut_q, cu_k, first_q, first_k, max_q, max_kv, scale, causal, left, sink_tokens)
+    kernel: prompt chunks are bound by its products, not by the cache.  As many sequences at a time as fit the buffers."""
+    C_ = _ext.get()
+    n, hq, d = page_table.shape[0], q.shape[1], q.shape[2]
+    group = max(1, _EXPAND_BYTES // _expansion_bytes(hq, cache.k.shape[1], d, max_q, max_kv))
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    for i in range(0, n, group):
+        table, cu, lens = (page_table, cu_q, kv_lens) if group >= n else \
+            (page_table[i:i + group], cu_q[i:i + group + 1], kv_lens[i:i + group])
+        k, v, cu_k, first_k, cut_q, first_q = C_.fp8_cache_expand(q, *cache, table, cu, lens, out, max_q, max_kv, left, sink_tokens,
+                                                                  i + group >= n)
+        _flash.flash_varlen_forward(q, k, v, out, cut_q, cu_k, first_q, first_k, max_q, max_kv, scale, causal, left, sink_tokens)
+        del k, v
+    return out
 
 
 def copy_pages(caches: Sequence[Union[torch.Tensor, FP8KVCache]], src: Union[Sequence[int], torch.Tensor],

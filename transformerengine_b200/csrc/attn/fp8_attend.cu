@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Tune<D, NT>::kCtas)) attend_kern
   __shared__ int sm_scan[kWarps], sm_at[2], sm_total;
   const Fp8AttendArgs& a = p.a;
   cudaTriggerProgrammaticLaunchCompletion();   // the joining kernel may be launched (it waits for this one's end)
-  zero_unclaimed(reinterpret_cast<uint32_t*>(a.out), static_cast<long long>(a.hq) * (D / 2), a.cu_q, a.c.n, a.tq, a.max_q,
+  zero_unclaimed(reinterpret_cast<uint32_t*>(a.out), static_cast<long long>(a.hq) * (D / 2), a.cu_q, a.c.n, a.tq, a.max_q, true,
                  static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x, static_cast<long long>(gridDim.x) * gridDim.y);
   if (a.c.n == 0) return;
   Run run;

@@ -29,11 +29,11 @@ __device__ __forceinline__ SeqFit fit_sequence(const int* cu_q, const int* kv_le
   return f;
 }
 
-// Zeros in the output rows (of `words` 32-bit words) that no query claims: behind the last sequence, and, reported by
-// fit_sequence, those of a sequence beyond max_q.  All threads of `ctas` CTAs take part.
+// Zeros in the output rows (of `words` 32-bit words) that no query claims: behind the last sequence (if `last`), and,
+// reported by fit_sequence, those of a sequence beyond max_q.  All threads of `ctas` CTAs take part.
 __device__ __forceinline__ void zero_unclaimed(uint32_t* out, long long words, const int* cu_q, int n, int tq, int max_q,
-                                               long long cta, long long ctas) {
-  const int end = cu_q[n];
+                                               bool last, long long cta, long long ctas) {
+  const int end = last ? cu_q[n] : tq;
   int q0 = cta < n ? cu_q[cta] : 0, q1 = cta < n ? cu_q[cta + 1] : 0;   // the first (mostly the only) turn of the loop below
   for (long long i = max(end, 0) * words + cta * blockDim.x + threadIdx.x; i < tq * words; i += ctas * blockDim.x) out[i] = 0u;
   for (long long seq = cta; seq < n;) {

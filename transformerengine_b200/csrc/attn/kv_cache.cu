@@ -194,7 +194,7 @@ __device__ __forceinline__ void store8<__half>(__half* p, const float (&y)[8]) {
 __device__ __forceinline__ void expansion_extras(const Fp8GatherArgs& a) {
   const long long cta = (static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
   const long long ctas = static_cast<long long>(gridDim.x) * gridDim.y * gridDim.z;
-  zero_unclaimed(static_cast<uint32_t*>(a.out), a.row_bytes / 4, a.cu_q, a.c.n, a.tq, a.max_q, cta, ctas);
+  zero_unclaimed(static_cast<uint32_t*>(a.out), a.row_bytes / 4, a.cu_q, a.c.n, a.tq, a.max_q, a.last, cta, ctas);
   if (cta != 0 || threadIdx.x >= 32) return;
   const int lane = threadIdx.x;
   int base = 0, base_q = 0;

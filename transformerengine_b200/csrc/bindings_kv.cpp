@@ -133,11 +133,12 @@ void fp8_cache_gather(const at::Tensor& k, const at::Tensor& v, const at::Tensor
   TORCH_CHECK(e == cudaSuccess, "fp8_cache_gather failed: ", cudaGetErrorString(e));
 }
 
-// Keys and values expanded for the packed attention kernel, pitch rows apart: {k, v, out, cumulative lengths and first rows
-// of the keys, those of the queries}; out has the rows that no query claims zeroed and waits for the others.
+// Keys and values expanded for the packed attention kernel, pitch rows apart: {k, v, cumulative lengths and first rows of the
+// keys, those of the queries}; rows of out that no query claims are zeroed (those behind the last query if `last`).
 std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
                                          const at::Tensor& vs, const at::Tensor& table, const at::Tensor& cu_q,
-                                         const at::Tensor& kv_lens, int64_t max_q, int64_t max_kv, int64_t window_left, int64_t sinks) {
+                                         const at::Tensor& kv_lens, const at::Tensor& out, int64_t max_q, int64_t max_kv,
+                                         int64_t window_left, int64_t sinks, bool last) {
   c10::cuda::CUDAGuard guard(k.device());
   teb200::Fp8GatherArgs a;
   a.c = cache_view(k, v, ks, vs, table, kv_lens);
@@ -149,7 +150,8 @@ std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& 
   TORCH_CHECK(pitch * a.c.n <= INT_MAX, "attend: sequences times max_kv is out of range");
   const at::Tensor ek = at::empty({pitch * a.c.n, a.c.heads, a.c.d}, q.options());
   const at::Tensor ev = at::empty_like(ek);
-  const at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  TORCH_CHECK(out.sizes() == q.sizes() && out.is_contiguous() && out.scalar_type() == q.scalar_type() && out.device() == q.device(),
+              "the output must be contiguous and like the queries");
   const at::Tensor meta = at::empty({4, a.c.n + 1}, cu_q.options());
   a.dtype = value_type(q, "queries");
   a.out_k = ek.data_ptr();
@@ -167,10 +169,11 @@ std::vector<at::Tensor> fp8_cache_expand(const at::Tensor& q, const at::Tensor& 
   a.max_q = static_cast<int>(std::min(max_q, q.size(0)));
   a.out = out.data_ptr();
   a.tq = static_cast<int>(q.size(0));
+  a.last = last;
   a.row_bytes = q.size(1) * q.size(2) * q.element_size();
   const cudaError_t e = teb200::fp8_cache_gather(a, cur_stream());
   TORCH_CHECK(e == cudaSuccess, "fp8_cache_expand failed: ", cudaGetErrorString(e));
-  return {ek, ev, out, meta.select(0, 0), meta.select(0, 1), meta.select(0, 2), meta.select(0, 3)};
+  return {ek, ev, meta.select(0, 0), meta.select(0, 1), meta.select(0, 2), meta.select(0, 3)};
 }
 
 at::Tensor fp8_cache_attend(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,

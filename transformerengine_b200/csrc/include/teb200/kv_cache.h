@@ -59,6 +59,7 @@ struct Fp8GatherArgs {
   int* first_q = nullptr;       // [n + 1]
   void* out = nullptr;          // [tq, row_bytes]
   int tq = 0;
+  bool last = true;             // the rows of `out` behind the last sequence are nobody's
   long long row_bytes = 0;      // multiple of 4
 };
 cudaError_t fp8_cache_gather(const Fp8GatherArgs& a, cudaStream_t stream);
