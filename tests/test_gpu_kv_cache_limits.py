@@ -233,3 +233,42 @@ def test_sequences_expanded_in_groups_give_the_same(monkeypatch):
         _litter(q)
         assert torch.equal(run(), want)
     te.check_status()
+
+
+@both_paths
+@pytest.mark.parametrize("how", ["address", "stride"])
+def test_queries_at_odd_addresses_and_strides(how, expand, monkeypatch):
+    _path(monkeypatch, expand)
+    lens, qs = [300, 200], [70, 5]
+    cache, table = _filled(lens, 2, 64, 128, torch.Generator().manual_seed(12))
+    q = _queries(sum(qs))
+    if how == "address":
+        odd = torch.zeros(q.numel() + 3, dtype=q.dtype, device="cuda")[3:].view(q.shape)
+    else:
+        odd = torch.zeros(sum(qs), 8, 132, dtype=q.dtype, device="cuda")[..., :128]
+    odd.copy_(q)
+    run = lambda x: kc.attend(x, cache, table, _i32(_cum(qs)), _i32(lens), max_q=70, max_kv=300)  # noqa: E731
+    assert torch.equal(run(odd), run(q))
+    te.check_status()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_training_attention_takes_tensors_at_odd_addresses(packed):
+    """Forward and backward, as from tensors where the kernels can read them in place."""
+    odd = lambda t: torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)  # noqa: E731
+    lens = [200, 57]
+    q, k, v, do = (_queries(sum(lens), h, seed=h + i) for i, h in enumerate((4, 2, 2, 4)))
+
+    def run(change):
+        x = [change(t).requires_grad_() for t in (q, k, v)]
+        if packed:
+            attn = te.DotProductAttention(4, 128, num_gqa_groups=2, qkv_format="thd", attn_mask_type="padding_causal", window_size=(60, 0),
+                                          sink_tokens=5).cuda()
+            o = attn(*x, cu_seqlens_q=_i32(_cum(lens)), cu_seqlens_kv=_i32(_cum(lens)))
+            return (o, *torch.autograd.grad(o, x, change(do).view_as(o)))
+        o = te.functional.attention(*(t.transpose(0, 1)[None] for t in x), causal=True, window=(60, 0), sink_tokens=5)
+        return (o, *torch.autograd.grad(o, x, change(do).transpose(0, 1)[None]))
+
+    for a, b in zip(run(odd), run(torch.clone)):
+        assert torch.equal(a, b)
+    te.check_status()

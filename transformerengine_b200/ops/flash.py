@@ -29,7 +29,8 @@ def supported(q, k, v, causal) -> bool:
 
 
 def _prep(t: torch.Tensor) -> torch.Tensor:
-    return t if _view_ok(t) else t.contiguous()
+    # (not contiguous(): that is the tensor itself where only the address does not fit)
+    return t if _view_ok(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _empty_out(q: torch.Tensor, out_format: str) -> torch.Tensor:
@@ -121,7 +122,7 @@ def supported_varlen(q, k, v) -> bool:
 def _thd_view(t: torch.Tensor) -> torch.Tensor:
     """[t, h, d] -> [1, h, t, d] view (copy only if the layout cannot be described to TMA)."""
     v = t.permute(1, 0, 2).unsqueeze(0)
-    return v if _view_ok(v) else t.contiguous().permute(1, 0, 2).unsqueeze(0)
+    return v if _view_ok(v) else t.clone(memory_format=torch.contiguous_format).permute(1, 0, 2).unsqueeze(0)
 
 
 class _FlashVarlenFunc(torch.autograd.Function):
