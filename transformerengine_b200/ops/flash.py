@@ -52,7 +52,7 @@ class _FlashFunc(torch.autograd.Function):
         s_pad = (sq + 127) // 128 * 128  # the backward reads lse / delta in blocks of 128 rows
         lse = torch.empty(b, h, s_pad, dtype=torch.float32, device=q.device)
         sc = float(scale) if scale is not None else d ** -0.5
-        wl, wr = (-1, -1) if window is None else (int(window[0]), int(window[1]))
+        wl, wr = _sides(window, sq, k.shape[2])
         # with sinks the backward also gets what rounding the output left over
         lo = torch.empty_like(out) if sink_tokens and any(ctx.needs_input_grad[:3]) else None
         C_.flash_fwd(q, k, v, out, lse, sc, bool(causal), bool(bottom_right), C_.status(q.device.index),
@@ -74,6 +74,14 @@ class _FlashFunc(torch.autograd.Function):
         C_.flash_bwd(dout, q, k, v, out, lse, delta, dq, dk, dv, sc, causal, bottom_right,
                      C_.status(q.device.index), window_left=wl, window_right=wr, sink_tokens=sink_tokens, out_lo=lo)
         return dq, dk, dv, None, None, None, None, None, None
+
+
+def _sides(window, sq: int, sk: int):
+    """Left and right side of a window (-1: open).  No key lies further than sq + sk from a query, so that longer sides are
+    cut there: the kernels hold them, and sums with lengths, in 32 bits."""
+    if window is None:
+        return -1, -1
+    return tuple(-1 if x < 0 else min(int(x), sq + sk) for x in window)
 
 
 def _sinks(window, sink_tokens: int, sk: int) -> int:
@@ -138,7 +146,7 @@ class _FlashVarlenFunc(torch.autograd.Function):
         sc = float(scale) if scale is not None else d ** -0.5
         qv, kv, vv = _thd_view(q), _thd_view(k), _thd_view(v)
         lo = torch.empty_like(out) if sink_tokens and any(ctx.needs_input_grad[:3]) else None
-        wl, wr = (-1, -1) if window is None else (int(window[0]), int(window[1]))
+        wl, wr = _sides(window, max_sq, max_sk)
         C_.flash_fwd_varlen(qv, kv, vv, _thd_view(out), lse, cu_q, cu_k, off_q, off_k, max_sq, max_sk, sc,
                             bool(causal), bool(bottom_right), C_.status(q.device.index), window_left=wl,
                             window_right=wr, sink_tokens=sink_tokens, out_lo=None if lo is None else _thd_view(lo))
@@ -167,9 +175,10 @@ def flash_varlen_forward(q, k, v, out, cu_q, cu_k, off_q, off_k, max_sq, max_sk,
     Rows outside every sequence are not written."""
     C_ = _ext.get()
     lse = torch.empty(cu_q.numel() - 1, q.shape[1], (max_sq + 127) // 128 * 128, dtype=torch.float32, device=q.device)
+    wl, wr = _sides((window_left, -1), max_sq, max_sk)
     C_.flash_fwd_varlen(_thd_view(q), _thd_view(k), _thd_view(v), _thd_view(out), lse, cu_q, cu_k, off_q, off_k, max_sq,
-                        max_sk, scale, bool(causal), True, C_.status(q.device.index), window_left=window_left,
-                        window_right=-1, sink_tokens=_sinks((window_left, -1), sink_tokens, max_sk))
+                        max_sk, scale, bool(causal), True, C_.status(q.device.index), window_left=wl,
+                        window_right=wr, sink_tokens=_sinks((window_left, -1), sink_tokens, max_sk))
     return out
 
 
