@@ -272,3 +272,37 @@ def test_training_attention_takes_tensors_at_odd_addresses(packed):
     for a, b in zip(run(odd), run(torch.clone)):
         assert torch.equal(a, b)
     te.check_status()
+
+
+# ------------------------------------------------------------------------------------------------------- accuracy
+@pytest.mark.parametrize("d,hq,n,qn", [(128, 8, 8000, 1), (64, 8, 3000, 4), (256, 4, 5000, 1), (128, 8, 600, 3)])
+@pytest.mark.parametrize("share", [0.999, 0.9999])
+def test_a_dominating_first_token_leaves_the_others_their_part(d, hq, n, qn, share):
+    """Token 0 takes almost all of the probability and has no value: what the others add up to is the result."""
+    g = torch.Generator().manual_seed(13)
+    table = _i32([list(range(-(-n // 64)))])
+    cache = kc.FP8KVCache.allocate(table.shape[1], 2, 64, d, device="cuda")
+    x = torch.randn(2, n, 2, d, generator=g)
+    x[0, :, :, 0], x[0, 0], x[1, 0] = 0.0, 0.0, 0.0
+    x[0, 0, :, 0] = 16.0
+    x = x.cuda()
+    kc.append(cache, x[0], x[1], table, _i32([0, n]), _i32([n]))
+    q = torch.randn(qn, hq, d, generator=g) * 0.5
+    q[..., 0] = math.log(share / (1 - share) * n) * math.sqrt(d) / 16.0
+    q = q.to(torch.bfloat16).cuda()
+    o = kc.attend(q, cache, table, _i32([0, qn]), _i32([n]), max_q=qn, max_kv=n).double()
+    dec = [c.float().double() * s.double().repeat_interleave(16, dim=2)[..., None] for c, s in
+           ((cache.k, cache.k_scale), (cache.v, cache.v_scale))]
+    k, v = (t[table[0].long()].transpose(0, 1).reshape(2, -1, d)[:, :n] for t in dec)
+    for a in range(hq):
+        s = q[:, a].double() @ k[a // (hq // 2)].T / math.sqrt(d)
+        pos = n - qn + torch.arange(qn, device="cuda")[:, None]
+        p = torch.softmax(s.masked_fill(torch.arange(n, device="cuda")[None] > pos, -math.inf), -1)
+        assert (p[:, 0] > share - 0.05).all()
+        want, mass = p @ v[a // (hq // 2)], p @ v[a // (hq // 2)].abs()
+        # the result and the probabilities (fp16) are rounded once; as much again as the latter for fp32 scores and sums;
+        # probabilities below 2^-29 of the largest lose up to 2^-40 of it
+        tol = 2.0 ** -8 * want.abs() + 2 * 2.0 ** -11 * mass + n * 2.0 ** -40 * 6.0
+        err = (o[:, a] - want).abs()
+        assert (err <= tol).all(), (err / tol).max()
+    te.check_status()

@@ -11,8 +11,10 @@
 // permuted in shared memory so that both reads are free of bank conflicts.
 // Codes become fp16 exactly.  Q is scaled per row by a power of two into fp16's range (bf16 has fewer bits than fp16, so
 // only values 2^-29 below the row's largest lose any).  A block's K scale multiplies its scores, its V scale s multiplies
-// the probabilities: with the running maximum m taken over score + log2 s, exp2(score + log2 s - m) stays within 1 and
-// fits fp16 whatever the scales (kept within 2^-60 .. 2^60); sums and accumulators are fp32.
+// the probabilities: with the running maximum m taken over score + log2 s, exp2(score + log2 s - m + 15) stays within 2^15
+// and fits fp16 whatever the scales (kept within 2^-60 .. 2^60); sums and accumulators are fp32.  The 15 bits keep what the
+// others add up to beside a token that takes nearly everything: without them codes below 2^-25 of the largest were zero in
+// the products but not in the row sum (8000 tokens beside a first one with 99.99 % of the mass: 13 % off, now 2^-11).
 // The steps of all sequences and heads form one line that the resident CTAs share equally, whatever the lengths: a CTA
 // walks the end of one sequence, whole ones, and the beginning of another, and a second kernel joins the sequences that
 // were cut.  Where no sequence is long (kDirectSteps), or a window makes them alike, a CTA per sequence and head takes it
@@ -42,6 +44,13 @@ constexpr int kWarps = 4;
 constexpr int kDirectSteps = 32;
 constexpr int kMinShare = 8;
 
+// Softmax offset of a row that has seen nothing: finite, so that differences with it are no NaN.
+constexpr float kNothingSeen = -3.4e38f;
+
+// What a row subtracts from its scores (log2) before the exponential: their maximum less 15.  Beyond 2^20, where the
+// subtraction would be rounded and exp2 might leave fp16's range, the maximum itself.
+__device__ __forceinline__ float softmax_offset(float top) { return fabsf(top) < 1048576.f ? top - 15.f : top; }
+
 struct AttendParams {
   Fp8AttendArgs a;
   int ctas;        // 0: one CTA per (sequence, key head, tile of rows); else they share the line of steps
@@ -49,7 +58,7 @@ struct AttendParams {
   int group;       // query heads per key head
   float scale_log2;
   // workspace of the cut sequences: two slots per CTA (its first run of steps, and a later one)
-  float2* part_ml;   // [2 ctas][R] running maximum and row sum
+  float2* part_ml;   // [2 ctas][R] softmax offset and row sum
   float* part_o;     // [2 ctas][R][d]
   int4* cuts;        // [ctas] the cut sequence that the CTA begins: sequence, first row, slot, last CTA; slot < 0: none
 };
@@ -216,7 +225,7 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
     for (int j = 0; j < MT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[t][j][e] = 0.f;
-    m_run[t][0] = m_run[t][1] = -INFINITY;
+    m_run[t][0] = m_run[t][1] = kNothingSeen;
     l_run[t][0] = l_run[t][1] = 0.f;
   }
 
@@ -396,8 +405,8 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
     }
     __syncwarp();                 // every lane has read the keys
     fetch(n + kStages, false);
-    // ---- softmax of x = score + log2(V scale); exp2(x - m) is what multiplies the V codes, and divided by the scale it is
-    // the term of the row sum
+    // ---- softmax of x = score + log2(V scale); exp2(x - offset) is what multiplies the V codes, and divided by the scale
+    // it is the term of the row sum
     const bool need_mask = !all_held || tok0 + STEP - 1 > hi_min || (tok0 < lo_max && tok0 + STEP > a.sinks);
     uint32_t pf[NT][NB][2];
 #pragma unroll
@@ -441,12 +450,11 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], off));
       }
-      float alpha[2], m_use[2];
+      float alpha[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float m_new = fmaxf(m_run[t][e], mx[e]);
-        m_use[e] = m_new == -INFINITY ? 0.f : m_new;
-        alpha[e] = ex2(m_run[t][e] - m_use[e]);
+        const float m_new = fmaxf(m_run[t][e], softmax_offset(mx[e]));
+        alpha[e] = ex2(m_run[t][e] - m_new);
         m_run[t][e] = m_new;
         l_run[t][e] *= alpha[e];
       }
@@ -456,7 +464,7 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
         float pv[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pv[e] = ex2(s[t][b][e] - m_use[e & 1]);
+          pv[e] = ex2(s[t][b][e] - m_run[t][e & 1]);
           l_run[t][e & 1] = fmaf(pv[e], inv, l_run[t][e & 1]);
         }
         const __half2 h0 = __floats2half2_rn(pv[0], pv[1]), h1 = __floats2half2_rn(pv[2], pv[3]);
@@ -552,11 +560,10 @@ __device__ __forceinline__ void attend_run(const AttendParams& p, const Walk& w,
     float m = sm_m[0][r];
 #pragma unroll
     for (int v = 1; v < kWarps; ++v) m = fmaxf(m, sm_m[v][r]);
-    const float m_use = m == -INFINITY ? 0.f : m;
     float l = 0.f, x0 = 0.f, x1 = 0.f, x2 = 0.f, x3 = 0.f;
 #pragma unroll
     for (int v = 0; v < kWarps; ++v) {
-      const float f = ex2(sm_m[v][r] - m_use);
+      const float f = ex2(sm_m[v][r] - m);
       l += sm_l[v][r] * f;
       const float4 y = *reinterpret_cast<const float4*>(sm_o + (v * R + r) * (D + 4) + d);
       x0 += y.x * f;
@@ -710,7 +717,6 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p) {
   for (int s = lane; s < parts; s += 32) m = fmaxf(m, p.part_ml[place_of(s)].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  const float m_use = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   float acc[D / 32];
 #pragma unroll
@@ -719,7 +725,7 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p) {
   for (int s = warp; s < parts; s += kW) {
     const int at = place_of(s);
     const float2 v = p.part_ml[at];
-    const float f = ex2(v.x - m_use);
+    const float f = ex2(v.x - m);
     l += v.y * f;
     const float* src = p.part_o + static_cast<long long>(at) * D + lane * 2;
 #pragma unroll
