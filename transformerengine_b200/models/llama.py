@@ -42,9 +42,9 @@ class LlamaConfig:
     embedding_scale: Optional[float] = None   # multiply the token embeddings (Gemma: sqrt(hidden_size))
     tie_embeddings: bool = False              # the output head shares the embedding table
     sliding_window: Optional[int] = None      # attend to the last N tokens only (Mistral)
-    sink_tokens: int = 0                      # ... and to the first N tokens (streaming attention)
     qk_norm: bool = False                     # RMSNorm over each head of q and k, before the rotation (Qwen3)
     qk_norm_eps: float = 1e-6
+    sink_tokens: int = 0                      # with sliding_window: the first N tokens stay visible (streaming attention)
 
     @staticmethod
     def llama3_8b(**kw) -> "LlamaConfig":
