@@ -581,17 +581,29 @@ cudaError_t flash_bwd_join(const FlashArgs& a, cudaStream_t stream) {
 cudaError_t flash_delta(const FlashArgs& a, cudaStream_t stream) {
   const long long rows = static_cast<long long>(a.b) * a.hq * a.sq;
   if (rows == 0) return cudaSuccess;
-  if (rows > 0xffffffffll - 64) return cudaErrorInvalidValue;
+  const long long per_entry = static_cast<long long>(a.hq) * a.sq;
+  constexpr long long kMost = 0xffffffffll - 64;   // rows are numbered in 32 bits
+  if (per_entry > kMost) return cudaErrorInvalidValue;
   if (a.o_ss % 4 || a.o_sh % 4 || a.o_sb % 4 || a.do_ss % 4 || a.do_sh % 4 || a.do_sb % 4) return cudaErrorInvalidValue;
   const int warps = 8;
   const long long per = static_cast<long long>(warps) * attn::kDeltaRows;
-  const unsigned grid = static_cast<unsigned>((rows + per - 1) / per);
-  attn::flash_delta_kernel<<<grid, warps * 32, 0, stream>>>(
-      reinterpret_cast<const uint16_t*>(a.out), reinterpret_cast<const uint16_t*>(a.out_lo),
-      reinterpret_cast<const uint16_t*>(a.dout), a.delta, a.b, a.hq, a.sq,
-      a.s_pad, a.o_sb, a.o_sh, a.o_ss, a.do_sb, a.do_sh, a.do_ss, a.is_bf16 ? 1 : 0, a.o_sh < a.o_ss ? 1 : 0, a.cu_q,
-      a.off_q);
-  return cudaGetLastError();
+  const uint16_t *out = reinterpret_cast<const uint16_t*>(a.out), *lo = reinterpret_cast<const uint16_t*>(a.out_lo),
+                 *dout = reinterpret_cast<const uint16_t*>(a.dout);
+  const int at_once = static_cast<int>(kMost / per_entry < a.b ? kMost / per_entry : a.b);
+  // many sequences, and a longest one far above the others, may have more: as many batch entries at a time as fit
+  for (int b0 = 0; b0 < a.b; b0 += at_once) {
+    const int nb = a.b - b0 < at_once ? a.b - b0 : at_once;
+    const unsigned grid = static_cast<unsigned>((nb * per_entry + per - 1) / per);
+    const bool packed = a.cu_q != nullptr;     // then the entries are sequences of one [1, h, t, d] view
+    const long long o0 = packed ? 0 : b0 * a.o_sb, d0 = packed ? 0 : b0 * a.do_sb;
+    attn::flash_delta_kernel<<<grid, warps * 32, 0, stream>>>(
+        out + o0, lo == nullptr ? lo : lo + o0, dout + d0, a.delta + b0 * static_cast<long long>(a.hq) * a.s_pad, nb, a.hq, a.sq,
+        a.s_pad, a.o_sb, a.o_sh, a.o_ss, a.do_sb, a.do_sh, a.do_ss, a.is_bf16 ? 1 : 0, a.o_sh < a.o_ss ? 1 : 0,
+        packed ? a.cu_q + b0 : nullptr, packed ? a.off_q + b0 : nullptr);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace teb200
