@@ -306,3 +306,20 @@ def test_a_dominating_first_token_leaves_the_others_their_part(d, hq, n, qn, sha
         err = (o[:, a] - want).abs()
         assert (err <= tol).all(), (err / tol).max()
     te.check_status()
+
+
+@pytest.mark.parametrize("max_kv", [None, 1, 2 ** 40])
+def test_gather_of_many_sequences_with_any_bound(max_kv):
+    """One long sequence among short ones: fewer CTAs than blocks, whatever bound sizes the launch."""
+    lens = [20000] + [17 + i % 50 for i in range(300)]
+    cache, table = _filled(lens, 8, 64, 64, torch.Generator().manual_seed(14))
+    rows = sum(lens)
+    k, v = kc.gather(cache, table, _i32(lens), _i32(_cum(lens)[:-1]), rows, torch.float32, max_kv=max_kv)
+    for i in (0, 1, 150, 300):
+        at = _cum(lens)[i]
+        pages = table[i][:-(-lens[i] // 64)].long()
+        for got, codes, scales in ((k, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
+            x = codes.view(torch.uint8)[pages].view(torch.float8_e4m3fn).float()
+            x = (x * scales[pages].repeat_interleave(16, dim=2)[..., None]).transpose(1, 2).reshape(-1, 8, 64)[:lens[i]]
+            assert torch.equal(got[at:at + lens[i]], x)                  # codes times powers of two: exact
+    te.check_status()

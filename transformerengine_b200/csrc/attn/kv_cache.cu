@@ -398,6 +398,14 @@ cudaError_t gather_d(const Fp8GatherArgs& a, dim3 grid, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+// CTAs along a sequence's 16-token blocks: those of the longest one, but no millions in all where that is a loose bound
+// or few sequences are long (the kernels walk on by the grid's height)
+int blocks_of(long long blocks, const Fp8CacheView& c) {
+  const long long most = 262144 / (static_cast<long long>((2 * c.heads + 3) / 4) * c.n) + 1;
+  blocks = blocks < 1 ? 1 : (blocks < most ? blocks : most);
+  return static_cast<int>(blocks < 65535 ? blocks : 65535);
+}
+
 bool view_ok(const Fp8CacheView& c) {
   return c.pages > 0 && c.heads > 0 && c.page_size >= kKvBlock && c.page_size % kKvBlock == 0 && c.n <= 65535 &&
          c.width > 0;
@@ -408,12 +416,8 @@ bool view_ok(const Fp8CacheView& c) {
 cudaError_t fp8_cache_append(const Fp8AppendArgs& a, cudaStream_t s) {
   if (!view_ok(a.c)) return cudaErrorInvalidValue;
   if (a.c.n == 0 || a.t == 0) return cudaSuccess;
-  int blocks = (a.max_new + kKvBlock - 2) / kKvBlock + 1;  // a run may start on a block's last row
-  const int per_block = (2 * a.c.heads + 3) / 4;
-  const long long most = 262144 / (static_cast<long long>(per_block) * a.c.n) + 1;   // (a loose max_new starts no millions of CTAs)
-  if (blocks > most) blocks = static_cast<int>(most);
-  if (blocks > 65535) blocks = 65535;
-  const dim3 grid(per_block, blocks, a.c.n);
+  const long long blocks = (static_cast<long long>(a.max_new) + kKvBlock - 2) / kKvBlock + 1;  // a run may start on a block's last row
+  const dim3 grid((2 * a.c.heads + 3) / 4, blocks_of(blocks, a.c), a.c.n);
   if (a.dtype == kFloat32) return append_d<float>(a, grid, s);
   if (a.dtype == kFloat16) return append_d<__half>(a, grid, s);
   if (a.dtype == kBFloat16) return append_d<__nv_bfloat16>(a, grid, s);
@@ -426,9 +430,7 @@ cudaError_t fp8_cache_gather(const Fp8GatherArgs& a, cudaStream_t s) {
   if (a.off == nullptr && (a.cu_q == nullptr || a.cu_k == nullptr || a.first_row == nullptr || a.cut_q == nullptr || a.first_q == nullptr ||
                            a.out == nullptr || a.row_bytes % 4 != 0 || static_cast<long long>(a.pitch) * a.c.n > a.rows))
     return cudaErrorInvalidValue;
-  int blocks = (a.max_kv + 127) / 128 * 8;
-  blocks = blocks < 1 ? 1 : (blocks > 65535 ? 65535 : blocks);
-  const dim3 grid((2 * a.c.heads + 3) / 4, blocks, a.c.n);
+  const dim3 grid((2 * a.c.heads + 3) / 4, blocks_of((static_cast<long long>(a.max_kv) + 127) / 128 * 8, a.c), a.c.n);
   if (a.dtype == kFloat32) return gather_d<float>(a, grid, s);
   if (a.dtype == kFloat16) return gather_d<__half>(a, grid, s);
   if (a.dtype == kBFloat16) return gather_d<__nv_bfloat16>(a, grid, s);

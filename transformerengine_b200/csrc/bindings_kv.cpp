@@ -128,7 +128,7 @@ void fp8_cache_gather(const at::Tensor& k, const at::Tensor& v, const at::Tensor
   TORCH_CHECK(off.numel() >= a.c.n, "offsets: one per sequence");
   a.off = int_vec(off, off.numel(), k.device(), "offsets");
   a.rows = static_cast<int>(out_k.size(0));
-  a.max_kv = static_cast<int>(max_kv);
+  a.max_kv = static_cast<int>(std::max<int64_t>(std::min<int64_t>(max_kv, a.rows), 0));   // no sequence has more rows
   const cudaError_t e = teb200::fp8_cache_gather(a, cur_stream());
   TORCH_CHECK(e == cudaSuccess, "fp8_cache_gather failed: ", cudaGetErrorString(e));
 }
