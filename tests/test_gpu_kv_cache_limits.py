@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import transformerengine_b200 as te
-from test_gpu_kv_cache import _cum, _filled, _i32
+from test_gpu_kv_cache import _check_attend, _cum, _filled, _i32, _oracle
 from transformerengine_b200.attention import kv_cache as kc
 
 pytestmark = pytest.mark.gpu
@@ -323,3 +323,19 @@ def test_gather_of_many_sequences_with_any_bound(max_kv):
             x = (x * scales[pages].repeat_interleave(16, dim=2)[..., None]).transpose(1, 2).reshape(-1, 8, 64)[:lens[i]]
             assert torch.equal(got[at:at + lens[i]], x)                  # codes times powers of two: exact
     te.check_status()
+
+
+# -------------------------------------------------------------------------------------------------- prompt chunks
+@pytest.mark.parametrize("d,hq,hk", [(64, 8, 2), (256, 4, 1), (128, 8, 2)])
+@pytest.mark.parametrize("qs,lens,window,sinks", [([700, 1, 129, 0, 1], [1500, 3000, 129, 64, 20], -1, 0),
+                                                  ([513, 2, 1, 300], [600, 2500, 7, 1000], 200, 5)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_chunks_beside_single_tokens_match_64_bits(d, hq, hk, qs, lens, window, sinks, dtype):
+    cache, table = _filled(lens, hk, 64, d, torch.Generator().manual_seed(d + len(qs)))
+    q = _queries(sum(qs) + 3, hq, d, dtype=dtype)
+    o = kc.attend(q, cache, table, _i32(_cum(qs)), _i32(lens), max_q=max(qs), max_kv=max(lens), window=(window, 0), sink_tokens=sinks)
+    te.check_status()
+    want, mass = _oracle(q, cache, table, qs, lens, window, sinks)
+    expanded = kc._expands(len(qs), hq, hk, d, max(qs), len(q), max(lens)) and d == 128
+    _check_attend(o, want, mass, lens, 6.0, torch.finfo(dtype).eps / 2 if expanded else 2.0 ** -11)
+    assert (o[sum(qs):] == 0).all()
