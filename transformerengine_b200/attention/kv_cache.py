@@ -197,7 +197,9 @@ def attend(q: torch.Tensor, cache: FP8KVCache, page_table: torch.Tensor, cu_q: t
     ``kv_lens[i]`` (bottom-right alignment).  ``window = (left, right)`` limits what the query at position p sees to keys
     ``p - left .. p``, plus the first ``sink_tokens`` tokens; -1 leaves a side open, and the right side is the causal
     one.  ``max_q`` / ``max_kv`` bound the queries and tokens of a sequence: a longer one is cut there and reported.  Rows
-    that see nothing, rows behind the last sequence, and rows that were cut off are zero.  There is no backward pass."""
+    that see nothing, rows behind the last sequence, and rows that were cut off are zero.  With fp16 queries, prompt chunks
+    at head dim 128 may read keys and values as fp16 (beyond 65504, in a cache filled from another type, they saturate).
+    There is no backward pass."""
     if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("attention over the 8-bit cache has no backward pass: call it under torch.no_grad()")
     left = -1

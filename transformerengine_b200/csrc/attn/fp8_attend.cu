@@ -18,8 +18,8 @@
 // The steps of all sequences and heads form one line that the resident CTAs share equally, whatever the lengths: a CTA
 // walks the end of one sequence, whole ones, and the beginning of another, and a second kernel joins the sequences that
 // were cut.  Where no sequence is long (kDirectSteps), or a window makes them alike, a CTA per sequence and head takes it
-// whole.  64 sequences of up to 8000 tokens, 32 / 8 heads, d 128: 0.56 GB of codes in 99 us; 4 of up to 130000, 64 / 8 heads:
-// 0.78 GB in 150 us (a copy moves 6.5 TB/s).
+// whole.  64 sequences of up to 8000 tokens, 32 / 8 heads, d 128: 0.56 GB of codes in 99 - 112 us; 4 of up to 130000, 64 / 8
+// heads: 0.78 GB in 134 - 157 us (a copy moves 6.5 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

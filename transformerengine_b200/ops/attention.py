@@ -128,9 +128,10 @@ def attention(q, k, v, *, scale=None, causal=False, window=None, attn_mask=None,
     of the sliding window; without a left side of ``window`` it changes nothing.  (``sink`` is another thing: the extra
     logit of ``softmax_type="learnable"``.)
 
-    On CUDA the fused flash kernel of this library handles the common case
-    (16-bit, no bias / arbitrary mask / dropout, head dim 64 or 128); everything
-    else runs the reference math, which autograd differentiates.
+    On CUDA the fused flash kernels of this library handle the common case (16-bit, head dim 128, no bias / arbitrary
+    mask / dropout; any window and sinks).  Other head dims without a window take PyTorch's
+    ``scaled_dot_product_attention``; everything else, sinks at other head dims among it, runs the reference math, which
+    autograd differentiates and whose fp32 scores take ``s_q * s_k`` per head.
     """
     if sink_tokens < 0:
         raise ValueError("sink_tokens must not be negative")
